@@ -338,6 +338,99 @@ int rl_decode_linear_set_stages(int stages);
  * last FP32 bit of the accumulated sum. Process-wide; affects later launches. */
 int rl_decode_linear_set_max_splits(int max_splits);
 
+/*
+ * Bounded-cache operators. A query at position p of its sequence sees only the first `sinks` tokens and the last
+ * `window` tokens up to and including p:  V(p) = { t <= p : t < sinks or t > p - window }  (window >= 1, sinks >= 0;
+ * a window that covers the sequence is plain causal attention). Shared by the three attention launchers below:
+ * head_dim 128, 1 to 8 KV heads with 1 to 8 query heads each, scale positive and finite, FP32 scores, statistics and
+ * accumulation, masking by SELECT (what invisible slots hold - NaN included - reaches no result), one FP16 rounding of
+ * the output. Pages that hold no visible token are not read, and neither are their block-table entries: a caller may
+ * have given them to other sequences. None of the four has a counterpart in the reference (full causal attention over
+ * a cache that only grows, src/kernels/kernels.cuh:125-187 there).
+ *
+ * Workspaces are the caller's: device memory, 16-byte aligned, of at least the size that the matching query names,
+ * ZEROED ONCE before its first use (every launch leaves it ready for the next one). Launches that may run at the same
+ * time - on several streams, or in graphs replayed on several streams - need a workspace each; launches ordered one
+ * after the other, captured or not, may share one, also with different shapes as long as it is large enough.
+ */
+
+/* Bytes of workspace for the two decode launchers below at these shapes (weights != 0: for
+ * rl_launch_paged_attention_decode_weights). Host arithmetic only. A workspace for the largest num_seqs and
+ * max_blocks_per_seq serves every smaller call with the same heads. */
+int rl_window_attention_workspace_bytes(int32_t num_seqs, int32_t max_blocks_per_seq, int32_t num_q_heads,
+                                        int32_t num_kv_heads, int32_t weights, size_t* bytes_out);
+
+/* Synchronises the device and reports (then clears) the error flag of the two decode launchers in `workspace`: 0 when
+ * every page load they waited for arrived, 1 when a bounded wait gave up (that launch's results are undefined). */
+int rl_window_attention_health(void* workspace, int* flag_out);
+
+/*
+ * rl_launch_paged_attention_decode with a sliding window and sinks: one query token per sequence, at position
+ * seq_len - 1, over the visible part of its cached tokens. Rows with seq_len <= 0 are not written; seq_lens are cut
+ * at max_blocks_per_seq * 16. q rows 4-byte aligned. With rl_attention_set_prologue_overlap on, its two rules hold here
+ * as well.
+ */
+int rl_launch_paged_window_attention_decode(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                                            const void* kv_pool_layer, const int32_t* block_tables,
+                                            const int32_t* seq_lens, int32_t num_seqs, int32_t max_blocks_per_seq,
+                                            int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                                            int32_t window, int32_t sinks, void* workspace, size_t workspace_bytes,
+                                            void* stream);
+
+/*
+ * Decode attention over the whole cache that also accumulates how much attention each cached token receives:
+ * out as above with every token visible, and for token t of a sequence of L, per KV head,
+ *   weights[page of t][kv head][slot of t]  =  (t == L - 1 ? 0 : its old value)  +  sum over the group's query heads of
+ *   their softmax probability of t.
+ * weights is FP32 [num_blocks, num_kv_heads, 16], paged like the pool and addressed through the same block tables. The
+ * newest token (t == L - 1, the one this step scattered) starts its sum here, so a page needs no clearing when decode
+ * appends to it; the entries of tokens that a prompt wrote are cleared by the caller. No atomics: each entry has one
+ * writer, so a page belongs to one sequence of the call, and results are the same in every run. Rows with
+ * seq_len <= 0 write nothing. One call enqueues two kernels.
+ */
+int rl_launch_paged_attention_decode_weights(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                                             const void* kv_pool_layer, const int32_t* block_tables,
+                                             const int32_t* seq_lens, int32_t num_seqs, int32_t max_blocks_per_seq,
+                                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                                             float* weights, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace rl_launch_paged_window_prefill_attention needs for a chunk on the current device's SM count
+ * (0 when it would not cut any (query tile, head) pair into runs). Host arithmetic only. */
+int rl_window_prefill_workspace_bytes(int32_t chunk_start, int32_t chunk_len, int32_t num_q_heads, int32_t window,
+                                      int32_t sinks, size_t* bytes_out);
+
+/*
+ * rl_launch_paged_prefill_attention with a sliding window and sinks: row i of the chunk, at position chunk_start + i,
+ * sees V(chunk_start + i). Only block-table entries of pages some row of the chunk sees are read. Same alignment rules
+ * (q, out and the pool slice 16-byte aligned, row strides multiples of 8); num_q_heads / num_kv_heads at most 8.
+ * workspace may be NULL (or smaller than the query names): then no (query tile, head) pair is cut into runs, which
+ * only costs time. Its bounded waits report through rl_prefill_attention_health.
+ */
+int rl_launch_paged_window_prefill_attention(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                                             const void* kv_pool_layer, const int32_t* block_table_row,
+                                             int32_t max_blocks_per_seq, int32_t chunk_start, int32_t chunk_len,
+                                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                                             int32_t window, int32_t sinks, void* workspace, size_t workspace_bytes,
+                                             void* stream);
+
+/*
+ * Evicts cached tokens by accumulated attention weight. Per sequence of L = seq_lens[s] tokens (cut at
+ * max_blocks_per_seq * 16) and per KV head on its own, L' = min(L, budget) tokens are kept: the first `sinks`, the last
+ * `recent`, and of the rest the budget - sinks - recent with the largest weight (equal weights: the lowest position;
+ * NaN counts below every number, -0 as +0). Kept tokens move in cache order to slots 0 .. L'-1 of the pages that
+ * dst_block_tables names - K row, V row and weight, bit for bit - and new_seq_lens[s] = L' (0 for L <= 0).
+ * kept[s][h][j] (int32 [num_seqs, num_kv_heads, budget]) is the slot that kept token j of head h had, -1 for j >= L'.
+ *   dst_block_tables == block_tables: in place (pages behind the first ceil(L' / 16) are then free to reuse).
+ *   any other dst_block_tables: its pages must be apart from every page of the source tables; the source stays as it is.
+ * In either case a page belongs to one sequence of the call. new_seq_lens may be seq_lens itself. Slots behind L' in the
+ * last destination page keep what they hold. Cached keys keep the rotation of their old positions: the caller goes on
+ * counting positions for RoPE apart from cache slots. head_dim a multiple of 8 up to 1024.
+ */
+int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int32_t* block_tables, int32_t max_blocks_per_seq,
+                       const int32_t* dst_block_tables, int32_t dst_max_blocks_per_seq, const int32_t* seq_lens,
+                       int32_t* new_seq_lens, int32_t* kept, int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t budget, int32_t sinks, int32_t recent, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

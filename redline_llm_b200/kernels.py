@@ -28,6 +28,9 @@ ABI_SYMBOLS = (
     "rl_decode_linear_set_max_splits", "rl_launch_qkv_rope_kv_scatter", "rl_launch_decode_advance",
     "rl_launch_paged_prefill_attention", "rl_prefill_attention_health", "rl_attention_test_wait_expiry", "rl_prefill_attention_set_split_blocks",
     "rl_prefill_attention_run_length",
+    "rl_window_attention_workspace_bytes", "rl_window_attention_health", "rl_launch_paged_window_attention_decode",
+    "rl_launch_paged_attention_decode_weights", "rl_window_prefill_workspace_bytes",
+    "rl_launch_paged_window_prefill_attention", "rl_launch_kv_evict",
 )
 
 
@@ -76,6 +79,17 @@ def lib() -> C.CDLL:
         L.rl_prefill_attention_set_split_blocks.argtypes = [C.c_int]
         L.rl_prefill_attention_run_length.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_int32)]
         L.rl_decode_linear_set_max_splits.argtypes = [C.c_int]
+        size = C.c_size_t
+        L.rl_window_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, C.POINTER(size)]
+        L.rl_window_attention_health.argtypes = [vp, C.POINTER(C.c_int)]
+        L.rl_launch_paged_window_attention_decode.argtypes = [vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, f32,
+                                                              i32, i32, vp, size, vp]
+        L.rl_launch_paged_attention_decode_weights.argtypes = [vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, f32,
+                                                               vp, vp, size, vp]
+        L.rl_window_prefill_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, C.POINTER(size)]
+        L.rl_launch_paged_window_prefill_attention.argtypes = [vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, f32,
+                                                               i32, i32, vp, size, vp]
+        L.rl_launch_kv_evict.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]
         for name in ABI_SYMBOLS[2:]:
             getattr(L, name).restype = C.c_int
         _lib = L
@@ -202,6 +216,91 @@ def launch_paged_prefill_attention(out, out_row_stride, q, q_row_stride, kv_pool
         _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_table_row.data_ptr(),
         max_blocks_per_seq, chunk_start, chunk_len, num_q_heads, num_kv_heads, head_dim, scale, _stream(stream)),
         "paged prefill attention")
+
+
+def _workspace(bytes_needed: int, device):
+    import torch
+    return torch.zeros(max(16, bytes_needed), dtype=torch.uint8, device="cuda" if device is None else device)
+
+
+def window_attention_workspace_bytes(num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads, weights=False) -> int:
+    out = C.c_size_t(0)
+    _check(lib().rl_window_attention_workspace_bytes(num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads,
+                                                     1 if weights else 0, C.byref(out)), "window attention workspace")
+    return int(out.value)
+
+
+def window_attention_workspace(num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads, weights=False, device=None):
+    """A zeroed workspace tensor for launch_paged_window_attention_decode, or with weights=True for
+    launch_paged_attention_decode_weights (and then for both). One per stream that such launches may run on at the
+    same time; launches in stream order share it."""
+    return _workspace(window_attention_workspace_bytes(num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads, weights),
+                      device)
+
+
+def window_attention_health(workspace) -> int:
+    """0 if every bounded wait of the decode launches on this workspace completed since the last query (synchronises)."""
+    flag = C.c_int(0)
+    _check(lib().rl_window_attention_health(workspace.data_ptr(), C.byref(flag)), "rl_window_attention_health")
+    return flag.value
+
+
+def launch_paged_window_attention_decode(out, out_row_stride, q, q_row_stride, kv_pool_layer, block_tables, seq_lens,
+                                         num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads, head_dim, scale,
+                                         window, sinks, workspace, stream=None, q_offset=0):
+    """launch_paged_attention_decode over the first `sinks` and the last `window` cached tokens of each sequence;
+    pages (and table entries) outside both are not read. 1 to 8 query heads per KV head."""
+    _check(lib().rl_launch_paged_window_attention_decode(
+        _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_tables.data_ptr(),
+        seq_lens.data_ptr(), num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads, head_dim, scale, window, sinks,
+        workspace.data_ptr(), workspace.nbytes, _stream(stream)), "paged window attention decode")
+
+
+def launch_paged_attention_decode_weights(out, out_row_stride, q, q_row_stride, kv_pool_layer, block_tables, seq_lens,
+                                          num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads, head_dim, scale,
+                                          weights, workspace, stream=None, q_offset=0):
+    """Decode attention over the whole cache that adds each cached token's softmax probabilities, summed over the
+    query heads of a group, to weights (float32 [num_blocks, num_kv_heads, 16], paged like the pool); the newest
+    token's entry is set, not added to."""
+    _check(lib().rl_launch_paged_attention_decode_weights(
+        _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_tables.data_ptr(),
+        seq_lens.data_ptr(), num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads, head_dim, scale, _ptr(weights),
+        workspace.data_ptr(), workspace.nbytes, _stream(stream)), "paged attention decode with weights")
+
+
+def window_prefill_workspace_bytes(chunk_start, chunk_len, num_q_heads, window, sinks) -> int:
+    out = C.c_size_t(0)
+    _check(lib().rl_window_prefill_workspace_bytes(chunk_start, chunk_len, num_q_heads, window, sinks, C.byref(out)),
+           "window prefill workspace")
+    return int(out.value)
+
+
+def window_prefill_workspace(chunk_start, chunk_len, num_q_heads, window, sinks, device=None):
+    """A workspace tensor for launch_paged_window_prefill_attention at this chunk."""
+    return _workspace(window_prefill_workspace_bytes(chunk_start, chunk_len, num_q_heads, window, sinks), device)
+
+
+def launch_paged_window_prefill_attention(out, out_row_stride, q, q_row_stride, kv_pool_layer, block_table_row,
+                                          max_blocks_per_seq, chunk_start, chunk_len, num_q_heads, num_kv_heads,
+                                          head_dim, scale, window, sinks, workspace=None, stream=None, q_offset=0):
+    """launch_paged_prefill_attention with a sliding window and sinks: row i sees the first `sinks` tokens and the
+    last `window` up to its own position. Without a workspace no work is cut across CTAs (slower, same function)."""
+    _check(lib().rl_launch_paged_window_prefill_attention(
+        _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_table_row.data_ptr(),
+        max_blocks_per_seq, chunk_start, chunk_len, num_q_heads, num_kv_heads, head_dim, scale, window, sinks,
+        _ptr(workspace), 0 if workspace is None else workspace.nbytes, _stream(stream)),
+        "paged window prefill attention")
+
+
+def launch_kv_evict(kv_pool_layer, weights, block_tables, max_blocks_per_seq, dst_block_tables, dst_max_blocks_per_seq,
+                    seq_lens, new_seq_lens, kept, num_seqs, num_kv_heads, head_dim, budget, sinks, recent, stream=None):
+    """Shrinks each sequence's cache to `budget` tokens per KV head: the first `sinks`, the last `recent` and the
+    heaviest of the rest, moved in cache order to the pages of dst_block_tables (the same tensor as block_tables: in
+    place). kept (int32 [num_seqs, num_kv_heads, budget]) receives the slots they had, -1 behind the last."""
+    _check(lib().rl_launch_kv_evict(
+        _ptr(kv_pool_layer), _ptr(weights), block_tables.data_ptr(), max_blocks_per_seq, dst_block_tables.data_ptr(),
+        dst_max_blocks_per_seq, seq_lens.data_ptr(), new_seq_lens.data_ptr(), kept.data_ptr(), num_seqs, num_kv_heads,
+        head_dim, budget, sinks, recent, _stream(stream)), "kv evict")
 
 
 def set_prefill_attention_split_blocks(blocks: int) -> None:

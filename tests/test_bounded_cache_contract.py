@@ -1,0 +1,114 @@
+"""The bounded-cache launchers' refusals and host arithmetic, through the C ABI without a device: every call here is
+answered before anything is launched."""
+import ctypes as C
+
+import pytest
+
+from redline_llm_b200 import kernels as K
+
+NULL, SHAPE, WORKSPACE, LARGE = -1, -2, -3, -4
+P = 4096          # a stand-in pointer: aligned, never dereferenced by a refused call
+
+
+def decode(**kw):
+    a = dict(out=P, os=1536, q=P, qs=2048, pool=P, tab=P, lens=P, n=4, mb=8, qh=12, kvh=2, d=128, scale=0.1, window=64,
+             sinks=4, ws=P, wb=1 << 40)
+    a.update(kw)
+    return K.lib().rl_launch_paged_window_attention_decode(a["out"], a["os"], a["q"], a["qs"], a["pool"], a["tab"],
+                                                           a["lens"], a["n"], a["mb"], a["qh"], a["kvh"], a["d"],
+                                                           a["scale"], a["window"], a["sinks"], a["ws"], a["wb"], None)
+
+
+def weights(**kw):
+    a = dict(out=P, os=1536, q=P, qs=2048, pool=P, tab=P, lens=P, n=4, mb=8, qh=12, kvh=2, d=128, scale=0.1, w=P, ws=P,
+             wb=1 << 40)
+    a.update(kw)
+    return K.lib().rl_launch_paged_attention_decode_weights(a["out"], a["os"], a["q"], a["qs"], a["pool"], a["tab"],
+                                                            a["lens"], a["n"], a["mb"], a["qh"], a["kvh"], a["d"],
+                                                            a["scale"], a["w"], a["ws"], a["wb"], None)
+
+
+def prefill(**kw):
+    a = dict(out=P, os=1536, q=P, qs=2048, pool=P, tab=P, mb=8, start=0, n=100, qh=12, kvh=2, d=128, scale=0.1,
+             window=64, sinks=4, ws=None, wb=0)
+    a.update(kw)
+    return K.lib().rl_launch_paged_window_prefill_attention(a["out"], a["os"], a["q"], a["qs"], a["pool"], a["tab"],
+                                                            a["mb"], a["start"], a["n"], a["qh"], a["kvh"], a["d"],
+                                                            a["scale"], a["window"], a["sinks"], a["ws"], a["wb"], None)
+
+
+def evict(**kw):
+    a = dict(pool=P, w=P, tab=P, mb=8, dst=2 * P, dmb=4, lens=P, new=P, kept=P, n=4, kvh=2, d=128, budget=64, sinks=4,
+             recent=16)
+    a.update(kw)
+    return K.lib().rl_launch_kv_evict(a["pool"], a["w"], a["tab"], a["mb"], a["dst"], a["dmb"], a["lens"], a["new"],
+                                      a["kept"], a["n"], a["kvh"], a["d"], a["budget"], a["sinks"], a["recent"], None)
+
+
+ATTENTION_SHAPES = [dict(d=64), dict(d=256), dict(kvh=0), dict(kvh=9, qh=9, os=9 * 128, qs=9 * 128), dict(kvh=-1),
+                    dict(qh=13), dict(qh=1), dict(qh=18, os=18 * 128, qs=18 * 128), dict(mb=0), dict(mb=-5), dict(os=1535),
+                    dict(qs=1000), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")),
+                    dict(scale=float("inf")), dict(scale=3.0e38), dict(pool=P + 8)]
+
+
+@pytest.mark.parametrize("call", [decode, weights, prefill])
+@pytest.mark.parametrize("change", ATTENTION_SHAPES)
+def test_shapes_the_attention_launchers_refuse(call, change):
+    if call is prefill and change.get("mb") in (0, -5):
+        change = dict(change, n=1)
+    assert call(**change) == SHAPE
+    assert K.lib().rl_last_error()
+
+
+@pytest.mark.parametrize("call", [decode, weights, prefill])
+@pytest.mark.parametrize("name", ["out", "q", "pool", "tab"])
+def test_null_pointers_are_refused(call, name):
+    assert call(**{name: None}) == NULL
+
+
+def test_refusals_of_one_launcher_only():
+    for call in (decode, weights):
+        assert call(lens=None) == NULL and call(ws=None) == NULL
+        assert call(qs=2047) == SHAPE and call(q=P + 2) == SHAPE and call(ws=P + 8) == SHAPE
+        assert call(mb=(1 << 26) + 1) == LARGE
+        assert call(wb=0) == WORKSPACE
+        need = K.window_attention_workspace_bytes(4, 8, 12, 2, weights=call is weights)
+        assert call(wb=need - 1) == WORKSPACE and b"workspace" in K.lib().rl_last_error()
+        assert call(n=0, out=None) == 0 and call(n=-3, out=None) == 0
+    assert weights(w=None) == NULL and weights(w=P + 2) == SHAPE
+    for call in (decode, prefill):
+        assert call(window=0) == SHAPE and call(window=-1) == SHAPE and call(sinks=-1) == SHAPE
+    assert prefill(n=0, out=None) == 0
+    assert prefill(start=-1) == SHAPE and prefill(n=129) == SHAPE and prefill(start=29) == SHAPE
+    assert prefill(start=2**31 - 1, n=2**31 - 1) == SHAPE
+    assert prefill(q=P + 8) == SHAPE and prefill(out=P + 8) == SHAPE and prefill(qs=2044) == SHAPE
+    assert prefill(os=1540) == SHAPE
+
+
+def test_evict_refusals():
+    for name in ("pool", "w", "tab", "dst", "lens", "new", "kept"):
+        assert evict(**{name: None}) == NULL
+    for change in (dict(kvh=0), dict(kvh=65536), dict(d=0), dict(d=4), dict(d=100), dict(d=1032), dict(mb=0), dict(dmb=0),
+                   dict(budget=0), dict(budget=-1), dict(sinks=-1), dict(recent=-1), dict(sinks=60, recent=5),
+                   dict(sinks=2**31 - 1, recent=2**31 - 1), dict(budget=65), dict(dst=P), dict(pool=P + 8), dict(w=P + 2)):
+        assert evict(**change) == SHAPE, change
+    assert evict(mb=(1 << 26) + 1) == LARGE and evict(dmb=(1 << 26) + 1) == LARGE
+    assert evict(n=0, pool=None) == 0 and evict(n=-1, pool=None) == 0
+
+
+def test_workspace_queries():
+    size = K.window_attention_workspace_bytes
+    assert 0 < size(1, 1, 1, 1) <= size(64, 1, 12, 2) <= size(64, 2048, 12, 2)
+    assert size(64, 2048, 12, 2, weights=True) >= size(64, 2048, 12, 2)
+    assert size(8, 100, 12, 2, weights=True) <= size(9, 100, 12, 2, weights=True) <= size(9, 101, 12, 2, weights=True)
+    assert size(0, 1, 12, 2) >= 0
+    for bad in ((-1, 1, 12, 2), (1, 0, 12, 2), (1, 1, 12, 9), (1, 1, 12, 0), (1, 1, 18, 2), (1, 1, 7, 2)):
+        with pytest.raises(K.KernelError):
+            size(*bad)
+    out = C.c_size_t(7)
+    L = K.lib()
+    for bad in ((-1, 1, 12, 1, 0), (0, -1, 12, 1, 0), (0, 1, 0, 1, 0), (0, 1, 12, 0, 0), (0, 1, 12, 1, -1)):
+        assert L.rl_window_prefill_workspace_bytes(*bad, C.byref(out)) == SHAPE and out.value == 0
+    assert L.rl_window_prefill_workspace_bytes(0, 1, 12, 1, 0, None) == NULL
+    assert L.rl_window_attention_workspace_bytes(1, 1, 12, 2, 0, None) == NULL
+    assert L.rl_window_attention_health(None, None) == NULL
