@@ -105,6 +105,8 @@ struct Params {
   int* error_flag;
   int n_tiles;        // query tiles of the chunk
   int split_blocks;   // longest run of key blocks one CTA takes
+  int window;         // a row at position p sees keys > p - window ...
+  int sinks;          // ... and keys < sinks (both only where kWindow)
   float* partials;    // one record of kPartialFloats per (head, work item) for pairs cut across CTAs
 };
 
@@ -214,6 +216,30 @@ __device__ __forceinline__ bool PairAny(int id, bool pred) {
   return any != 0;
 }
 
+// The keys a query tile (rows at positions first .. last) needs under a sliding window with sinks, as a list of pages
+// without gaps: `sink_pages` pages from the start of the sequence, then the pages from `window_page` - which holds the
+// oldest key in any row's window - to the one of `last`. (Where the two meet they are one run from page 0.) Blocks of 8
+// pages are cut from that LIST, so neither end of the window costs more than a page of padding. A window that covers
+// the sequence gives the plain causal list: no sink pages, window_page 0.
+struct TileSpan {
+  int sink_pages, window_page, blocks;
+};
+__host__ __device__ __forceinline__ TileSpan SpanOfTile(int first, int last, int window, int sinks) {
+  const int oldest = first - window + 1 > 0 ? first - window + 1 : 0;
+  TileSpan s;
+  s.window_page = oldest >> kKvBlockShift;
+  const int pages = sinks > 0 ? ((sinks - 1) >> kKvBlockShift) + 1 : 0;
+  s.sink_pages = pages < s.window_page ? pages : s.window_page;
+  s.blocks = (s.sink_pages + (last >> kKvBlockShift) - s.window_page) / kPagesPerBlock + 1;
+  return s;
+}
+// Which of the 16 keys of a page starting at position `base` a row sees: bit i for key base + i.
+__device__ __forceinline__ uint32_t Below(int n) { return n >= 16 ? 0xFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t VisibleKeys(int base, int pos, int window, int sinks) {
+  return Below(pos + 1 - base) & (Below(sinks - base) | ~Below(pos - window + 1 - base));
+}
+
+template <bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1)
 PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap q_map,
                             const __grid_constant__ CUtensorMap page_map) {
@@ -279,7 +305,8 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
     bool found = false;
     for (int base = 0; base < p.n_tiles && !found; base += 32) {
       const int t = p.n_tiles - 1 - base - lane;
-      const int nb = t >= 0 ? (min(p.chunk_start + (t + 1) * kBM, kv_len) - 1) / kBN + 1 : 0;
+      const int last = min(p.chunk_start + (t + 1) * kBM, kv_len) - 1;
+      const int nb = t < 0 ? 0 : kWindow ? SpanOfTile(p.chunk_start + t * kBM, last, p.window, p.sinks).blocks : last / kBN + 1;
       const int ns = t >= 0 ? (nb + p.split_blocks - 1) / p.split_blocks : 0;
       int upto = ns;                      // inclusive scan over the lanes
 #pragma unroll
@@ -300,7 +327,7 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
     }
     if (!found) {                         // an item past the last one: the launcher never asks for it
       tile_q = 0;
-      tile_blocks = (min(p.chunk_start + kBM, kv_len) - 1) / kBN + 1;
+      tile_blocks = 1;
       nsplit = 1;
       split = 0;
     }
@@ -308,10 +335,22 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
   const int row0 = tile_q * kBM;
   const int jb0 = split * tile_blocks / nsplit;
   const int nblk = (split + 1) * tile_blocks / nsplit - jb0;          // blocks of THIS item, indexed 0 .. nblk - 1 below
+  // With a window, block and key indices count the tile's page list; entry i of the list is page i, or i + page_skip
+  // behind the sinks.
+  const int last_pos = min(p.chunk_start + row0 + kBM, kv_len) - 1;
+  int sink_pages = 0, page_skip = 0;
+  if (kWindow) {
+    const TileSpan span = SpanOfTile(p.chunk_start + row0, last_pos, p.window, p.sinks);
+    sink_pages = span.sink_pages;
+    page_skip = span.window_page - span.sink_pages;
+  }
+  auto key_pos = [&](int key) { return kWindow && key >= sink_pages * kKvBlock ? key + page_skip * kKvBlock : key; };
 
   // The loader's first table reads (lane l < 8 serves page l of a block) are under way before the CTA's barrier.
   auto table_entry = [&](int j) {
-    const int page = (jb0 + j) * kPagesPerBlock + lane;
+    const int entry = (jb0 + j) * kPagesPerBlock + lane;
+    const int page = kWindow && entry >= sink_pages ? entry + page_skip : entry;
+    if (kWindow && page > last_pos >> kKvBlockShift) return 0;   // behind the list: the dummy block
     return (lane < kPagesPerBlock && j < nblk && page < p.max_blocks) ? __ldg(p.table_row + page) : 0;   // past the table: the dummy block
   };
   int blk = 0, blk_next = 0, blk_next2 = 0;
@@ -467,7 +506,18 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
     for (int j = 0; j < nblk; ++j) {
       const int buf = j & 1;
       const int key0 = (jb0 + j) * kBN + hw * kKeysPerThread;
-      const bool diagonal = (jb0 + j) * kBN + kBN - 1 > p.chunk_start + row0;   // some row of the tile is masked inside this block
+      // some row of the tile is masked inside this block
+      bool diagonal = (jb0 + j) * kBN + kBN - 1 > p.chunk_start + row0;
+      uint32_t seen[kScoreChunks];   // kWindow: this row's visible keys, one 16-bit mask per chunk (a chunk is a page)
+      if (kWindow) {
+        const int first_key = key_pos((jb0 + j) * kBN), last_key = key_pos((jb0 + j) * kBN + kBN - 1);
+        diagonal = last_key > p.chunk_start + row0 || (first_key <= last_pos - p.window && last_key >= p.sinks);
+        if (diagonal) {
+#pragma unroll
+          for (int c = 0; c < kScoreChunks; ++c) seen[c] = VisibleKeys(key_pos(key0 + c * 16), my_pos, p.window, p.sinks);
+        }
+      }
+      auto visible = [&](int c, int i) { return kWindow ? ((seen[c] >> i) & 1u) != 0 : key0 + c * 16 + i <= my_pos; };
       const uint32_t p_addr = tmem_base + kTmemP + buf * (kBN / 2) + lane_addr + (kKeysPerThread / 2) * hw;
       const int pair_bar = 2 + (warp & 3);
       // The raw maximum of this thread's 64 scores (raw: the scale is positive), masked keys left out.
@@ -478,7 +528,7 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
           for (int c = 0; c < kScoreChunks; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              mx = fmaxf(mx, key0 + c * 16 + i <= my_pos ? __uint_as_float(raw[c][i]) : -INFINITY);
+              mx = fmaxf(mx, visible(c, i) ? __uint_as_float(raw[c][i]) : -INFINITY);
         } else {
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // four chains, two scores per instruction
 #pragma unroll
@@ -504,8 +554,8 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
             float p0 = Ex2(x.x);
             float p1 = Ex2(x.y);
             if (diagonal) {
-              p0 = key0 + c * 16 + i <= my_pos ? p0 : 0.0f;
-              p1 = key0 + c * 16 + i + 1 <= my_pos ? p1 : 0.0f;
+              p0 = visible(c, i) ? p0 : 0.0f;
+              p1 = visible(c, i + 1) ? p1 : 0.0f;
             }
             sums = Add2(sums, Pack2(p0, p1));
             packed[i >> 1] = AsU32(__floats2half2_rn(p0, p1));
@@ -568,10 +618,22 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
       l += sum;
       // V rows at or past the context end (the last block only) may hold anything, NaN included, and 0 * NaN
       // would poison the row: clear them once the block has landed.
-      const int rows_valid = kv_len - (jb0 + j) * kBN;
-      if (rows_valid < kBN) {
+      // (With a window: every key that no row of the tile sees - behind the last row, and between the sinks and the
+      // oldest key of the window in the pages that hold those two ends.)
+      bool clear_block, clear_row;
+      if (kWindow) {
+        const int b0 = (jb0 + j) * kBN, pos = key_pos(b0 + row);
+        clear_block = key_pos(b0 + kBN - 1) > last_pos ||
+                      (b0 <= sink_pages * kKvBlock + kKvBlock - 1 && b0 + kBN > (sink_pages - 1) * kKvBlock);
+        clear_row = pos > last_pos || (pos >= p.sinks && pos <= p.chunk_start + row0 - p.window);
+      } else {
+        const int rows_valid = kv_len - (jb0 + j) * kBN;
+        clear_block = rows_valid < kBN;
+        clear_row = row >= rows_valid;
+      }
+      if (clear_block) {
         wait(bar_v0 + 8 * buf, (j >> 1) & 1);
-        if (row >= rows_valid) {
+        if (clear_row) {
           // key `row` of the block: page row / 16, token group (row / 8) % 2, token row % 8; the row's threads
           // clear its 256 bytes between them (the swizzle only permutes 16-byte pieces inside a 128-byte row, and
           // all of them are cleared)
@@ -671,6 +733,7 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
 constexpr int kCombineThreads = 256;
 constexpr int kCombineRows = 32;
 static_assert(kCombineThreads / 32 * 16 == kHeadDim, "one warp per 16 dims");
+template <bool kWindow>
 __global__ void __launch_bounds__(kCombineThreads)
 PrefillCombineKernel(const Params p, int items) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -678,7 +741,8 @@ PrefillCombineKernel(const Params p, int items) {
   const int kv_len = p.chunk_start + p.chunk_len;
   int runs = 1, item0 = 0;   // the pair's runs and its first work item: the items of later tiles come first
   for (int t = p.n_tiles - 1; t >= tile; --t) {
-    const int nb = (min(p.chunk_start + (t + 1) * kBM, kv_len) - 1) / kBN + 1;
+    const int last = min(p.chunk_start + (t + 1) * kBM, kv_len) - 1;
+    const int nb = kWindow ? SpanOfTile(p.chunk_start + t * kBM, last, p.window, p.sinks).blocks : last / kBN + 1;
     runs = (nb + p.split_blocks - 1) / p.split_blocks;
     if (t > tile) item0 += runs;
   }
@@ -759,22 +823,33 @@ int g_split_blocks = 0;   // 0: chosen per launch (ChooseSplitBlocks); > 0: forc
 // items in two waves into 240 that level out, 120 -> 104 us); a prompt's last 128 rows against 32768 keys are cut
 // into a dozen runs each (263 -> 37 us). The choice depends on the chunk alone, so it is remembered across the
 // layers of a model.
-double SimulatedMakespan(int chunk_start, int chunk_len, int heads, int split_blocks, int sm_count, std::vector<double>& free_at) {
+// Key blocks of query tile t; window = INT32_MAX and sinks = 0 for plain causal attention.
+struct Chunk {
+  int start, len, heads, window, sinks;
+  int Tiles() const { return (len + kBM - 1) / kBM; }
+  int Blocks(int t) const {
+    const int64_t first = static_cast<int64_t>(start) + static_cast<int64_t>(t) * kBM;
+    const int64_t last = std::min<int64_t>(first + kBM, static_cast<int64_t>(start) + len) - 1;
+    return SpanOfTile(static_cast<int>(first), static_cast<int>(last), window, sinks).blocks;
+  }
+  bool operator==(const Chunk& o) const {
+    return start == o.start && len == o.len && heads == o.heads && window == o.window && sinks == o.sinks;
+  }
+};
+
+double SimulatedMakespan(const Chunk& chunk, int split_blocks, int sm_count, std::vector<double>& free_at) {
   constexpr double kBlockUs = 1.15, kSetupUs = 8.0, kPublishUs = 1.5, kCombineUs = 4.0;
-  const int64_t kv_len = static_cast<int64_t>(chunk_start) + chunk_len;
-  const int n_tiles = (chunk_len + kBM - 1) / kBM;
   free_at.assign(sm_count, 0.0);                       // a min-heap of the times at which the SMs free up
   double end = 0.0;
   bool any_cut = false;
-  for (int t = n_tiles - 1; t >= 0; --t) {
-    const int64_t last = std::min<int64_t>(static_cast<int64_t>(chunk_start) + static_cast<int64_t>(t + 1) * kBM, kv_len) - 1;
-    const int nb = static_cast<int>(last / kBN) + 1;
+  for (int t = chunk.Tiles() - 1; t >= 0; --t) {
+    const int nb = chunk.Blocks(t);
     const int ns = (nb + split_blocks - 1) / split_blocks;
     for (int run = 0; run < ns; ++run) {
       const int blocks = (run + 1) * nb / ns - run * nb / ns;
       const double cost = kSetupUs + blocks * kBlockUs + (ns > 1 ? kPublishUs : 0.0);
       any_cut |= ns > 1;
-      for (int h = 0; h < heads; ++h) {
+      for (int h = 0; h < chunk.heads; ++h) {
         std::pop_heap(free_at.begin(), free_at.end(), std::greater<double>());
         const double done = free_at.back() + cost;
         free_at.back() = done;
@@ -786,24 +861,25 @@ double SimulatedMakespan(int chunk_start, int chunk_len, int heads, int split_bl
   return end + (any_cut ? kCombineUs : 0.0);
 }
 
-int ChooseSplitBlocks(int chunk_start, int chunk_len, int heads, int sm_count) {
-  struct Memo { int start, len, heads, sms, choice; };
-  static Memo memo = {-1, -1, -1, -1, 0};
+int ChooseSplitBlocks(const Chunk& chunk, int sm_count) {
+  struct Memo { Chunk chunk; int sms, choice; };
+  static Memo memo = {{-1, -1, -1, -1, -1}, -1, 0};
   static std::mutex memo_mutex;
   std::lock_guard<std::mutex> lock(memo_mutex);
-  if (memo.start == chunk_start && memo.len == chunk_len && memo.heads == heads && memo.sms == sm_count) return memo.choice;
-  const int max_blocks = static_cast<int>((static_cast<int64_t>(chunk_start) + chunk_len - 1) / kBN) + 1;
-  const int n_tiles = (chunk_len + kBM - 1) / kBM;
+  if (memo.chunk == chunk && memo.sms == sm_count) return memo.choice;
+  const int n_tiles = chunk.Tiles(), heads = chunk.heads;
+  int max_blocks = 1;
+  for (int t = 0; t < n_tiles; ++t) max_blocks = std::max(max_blocks, chunk.Blocks(t));
   std::vector<double> heap;
   int best = max_blocks;
-  double best_us = SimulatedMakespan(chunk_start, chunk_len, heads, max_blocks, sm_count, heap);   // every pair whole
+  double best_us = SimulatedMakespan(chunk, max_blocks, sm_count, heap);   // every pair whole
   // A chunk that fills the machine many times over gains nothing from cuts, and replaying it would cost more than it saves.
   if (static_cast<int64_t>(n_tiles) * heads <= 6LL * sm_count) {
     const int64_t pairs = static_cast<int64_t>(n_tiles) * heads;
     auto consider = [&](int run) {
       if (run < 4 || run >= max_blocks) return;
       if (pairs * ((max_blocks + run - 1) / run) > 8LL * sm_count) return;   // bounds the replay at ~1200 items
-      const double us = SimulatedMakespan(chunk_start, chunk_len, heads, run, sm_count, heap);
+      const double us = SimulatedMakespan(chunk, run, sm_count, heap);
       if (us < best_us) {
         best_us = us;
         best = run;
@@ -812,7 +888,7 @@ int ChooseSplitBlocks(int chunk_start, int chunk_len, int heads, int sm_count) {
     for (int r : {2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32}) consider((max_blocks + r - 1) / r);   // equal cuts of the longest tile
     for (int run = max_blocks - 4; run > max_blocks / 2; run -= 4) consider(run);                   // cuts that only the longer tiles get
   }
-  memo = {chunk_start, chunk_len, heads, sm_count, best};
+  memo = {chunk, sm_count, best};
   return best;
 }
 
@@ -835,8 +911,10 @@ int EnsureReady(DeviceState** out_state) {
   if (CurrentDeviceFacts().max_smem_optin < kSmemBytes)
     return Fail(RL_E_WORKSPACE, "paged_prefill_attention: device offers %d B of shared memory per block, %d needed",
                 CurrentDeviceFacts().max_smem_optin, kSmemBytes);
-  cudaError_t e = cudaFuncSetAttribute(PagedPrefillAttentionKernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(PagedPrefillAttentionKernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        kSmemBytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(PagedPrefillAttentionKernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return Fail(static_cast<int>(e), "paged_prefill_attention: shared-memory opt-in: %s", cudaGetErrorString(e));
   e = cudaMalloc(reinterpret_cast<void**>(&st.error_flag), 256);
   if (e == cudaSuccess) e = cudaMemset(st.error_flag, 0, 256);
@@ -845,30 +923,48 @@ int EnsureReady(DeviceState** out_state) {
   return RL_OK;
 }
 
-}  // namespace pfa
-}  // namespace rl
+constexpr int kWholeWindow = INT32_MAX;
+// Window and sinks cut at the sequence: nothing changes, and sums of positions with them stay inside 32 bits.
+Chunk WindowChunk(int start, int len, int heads, int window, int sinks) {
+  return Chunk{start, len, heads, std::min(window, start + len), std::min(sinks, start + len)};
+}
 
-extern "C" int rl_launch_paged_prefill_attention(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
-                                                 const void* kv_pool_layer, const int32_t* block_table_row,
-                                                 int32_t max_blocks_per_seq, int32_t chunk_start, int32_t chunk_len,
-                                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                                                 float scale, void* stream) {
-  using namespace rl;
-  using namespace rl::pfa;
-  if (chunk_len <= 0) return RL_OK;
-  if (!out || !q || !kv_pool_layer || !block_table_row)
-    return Fail(RL_E_NULL_POINTER, "paged_prefill_attention: null device pointer");
-  if (head_dim != kHeadDim) return Fail(RL_E_BAD_SHAPE, "paged_prefill_attention: head_dim must be 128");
-  if (num_kv_heads < 1 || num_kv_heads > 8 || num_q_heads < num_kv_heads || num_q_heads % num_kv_heads != 0)
-    return Fail(RL_E_BAD_SHAPE, "paged_prefill_attention: num_q_heads must be a positive multiple of num_kv_heads (<= 8 KV heads)");
-  if (chunk_start < 0 || max_blocks_per_seq < 1 ||
-      static_cast<int64_t>(chunk_start) + chunk_len > static_cast<int64_t>(max_blocks_per_seq) * kKvBlock)
-    return Fail(RL_E_BAD_SHAPE, "paged_prefill_attention: the chunk runs past the block table row");
-  const int64_t width = static_cast<int64_t>(num_q_heads) * head_dim;
+int CheckChunk(const char* fn, const void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride, const void* pool,
+               const int32_t* table_row, int max_blocks, int chunk_start, int chunk_len, int q_heads, int kv_heads, int head_dim) {
+  if (!out || !q || !pool || !table_row) return Fail(RL_E_NULL_POINTER, "%s: null device pointer", fn);
+  if (head_dim != kHeadDim) return Fail(RL_E_BAD_SHAPE, "%s: head_dim must be 128", fn);
+  if (kv_heads < 1 || kv_heads > 8 || q_heads < kv_heads || q_heads % kv_heads != 0)
+    return Fail(RL_E_BAD_SHAPE, "%s: num_q_heads must be a positive multiple of num_kv_heads (<= 8 KV heads)", fn);
+  if (chunk_start < 0 || max_blocks < 1 ||
+      static_cast<int64_t>(chunk_start) + chunk_len > static_cast<int64_t>(max_blocks) * kKvBlock)
+    return Fail(RL_E_BAD_SHAPE, "%s: the chunk runs past the block table row", fn);
+  const int64_t width = static_cast<int64_t>(q_heads) * head_dim;
   if (q_row_stride < width || out_row_stride < width)
-    return Fail(RL_E_BAD_SHAPE, "paged_prefill_attention: row stride smaller than the row");
-  if ((q_row_stride & 7) || (out_row_stride & 7) || !Aligned16(q) || !Aligned16(out) || !Aligned16(kv_pool_layer))
-    return Fail(RL_E_BAD_SHAPE, "paged_prefill_attention: q, out and the pool slice must be 16-byte aligned with row strides in multiples of 8");
+    return Fail(RL_E_BAD_SHAPE, "%s: row stride smaller than the row", fn);
+  if ((q_row_stride & 7) || (out_row_stride & 7) || !Aligned16(q) || !Aligned16(out) || !Aligned16(pool))
+    return Fail(RL_E_BAD_SHAPE, "%s: q, out and the pool slice must be 16-byte aligned with row strides in multiples of 8", fn);
+  return RL_OK;
+}
+
+// Work items of a head when no run is longer than split_blocks key blocks, and how many of the chunk's last tiles lie
+// at or behind the first one that is cut (0: none is).
+int64_t CountItems(const Chunk& chunk, int split_blocks, int* cut_tiles) {
+  int64_t items = 0;
+  *cut_tiles = 0;
+  for (int t = chunk.Tiles() - 1; t >= 0; --t) {
+    const int ns = (chunk.Blocks(t) + split_blocks - 1) / split_blocks;
+    items += ns;
+    if (ns > 1) *cut_tiles = chunk.Tiles() - t;
+  }
+  return items;
+}
+
+template <bool kWindow>
+int LaunchChunk(const char* fn, void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                const void* kv_pool_layer, const int32_t* block_table_row, int max_blocks_per_seq, const Chunk& chunk,
+                int num_kv_heads, float scale, float* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  const int num_q_heads = chunk.heads, chunk_start = chunk.start, chunk_len = chunk.len;
+  const int64_t width = static_cast<int64_t>(num_q_heads) * kHeadDim;
   DeviceState* st;
   int rc = EnsureReady(&st);
   if (rc != RL_OK) return rc;
@@ -881,7 +977,7 @@ extern "C" int rl_launch_paged_prefill_attention(void* out, int64_t out_row_stri
     const CUresult r = g_encode(&q_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(q), dims, strides, box, estr,
                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return Fail(RL_E_BAD_SHAPE, "paged_prefill_attention: q tensor map (CUresult %d)", static_cast<int>(r));
+    if (r != CUDA_SUCCESS) return Fail(RL_E_BAD_SHAPE, "%s: q tensor map (CUresult %d)", fn, static_cast<int>(r));
   }
   {
     // The pool slice as [tile][token group of 8][dim half][token in group][64 halves] (strides 4096, 2048, 128, 256,
@@ -896,26 +992,23 @@ extern "C" int rl_launch_paged_prefill_attention(void* out, int64_t out_row_stri
     const CUresult r = g_encode(&page_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(kv_pool_layer), dims, strides,
                                 box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return Fail(RL_E_BAD_SHAPE, "paged_prefill_attention: pool tensor map (CUresult %d)", static_cast<int>(r));
+    if (r != CUDA_SUCCESS) return Fail(RL_E_BAD_SHAPE, "%s: pool tensor map (CUresult %d)", fn, static_cast<int>(r));
   }
   // Work items per head: a tile with more than split_blocks key blocks is cut into ceil(blocks / split_blocks) runs.
-  const int split_blocks = g_split_blocks > 0 ? g_split_blocks
-                                              : ChooseSplitBlocks(chunk_start, chunk_len, num_q_heads, CurrentDeviceFacts().sm_count);
-  const int n_tiles = (chunk_len + kBM - 1) / kBM;
-  const int64_t kv_len = static_cast<int64_t>(chunk_start) + chunk_len;
-  int64_t items = 0;
-  bool any_split = false;
-  for (int t = 0; t < n_tiles; ++t) {
-    const int64_t last = (static_cast<int64_t>(chunk_start) + static_cast<int64_t>(t + 1) * kBM < kv_len
-                              ? static_cast<int64_t>(chunk_start) + static_cast<int64_t>(t + 1) * kBM
-                              : kv_len) - 1;
-    const int nb = static_cast<int>(last / kBN) + 1;
-    const int ns = (nb + split_blocks - 1) / split_blocks;
-    items += ns;
-    any_split |= ns > 1;
+  int split_blocks = g_split_blocks > 0 ? g_split_blocks : ChooseSplitBlocks(chunk, CurrentDeviceFacts().sm_count);
+  int cut_tiles;
+  int64_t items = CountItems(chunk, split_blocks, &cut_tiles);
+  float* partials = nullptr;
+  if (kWindow && cut_tiles > 0) {
+    partials = workspace;
+    if (!workspace || workspace_bytes < static_cast<size_t>(num_q_heads) * items * kPartialFloats * sizeof(float)) {
+      split_blocks = INT32_MAX / 2;   // no room for the runs' records: every pair whole
+      items = CountItems(chunk, split_blocks, &cut_tiles);
+    }
   }
-  if (items > 65535) return Fail(RL_E_TOO_LARGE, "paged_prefill_attention: chunk too large (%lld work items per head)", static_cast<long long>(items));
-  if (any_split) {
+  const bool any_split = cut_tiles > 0;
+  if (items > 65535) return Fail(RL_E_TOO_LARGE, "%s: chunk too large (%lld work items per head)", fn, static_cast<long long>(items));
+  if (any_split && !kWindow) {
     const size_t need = static_cast<size_t>(num_q_heads) * static_cast<size_t>(items) * kPartialFloats;
     std::lock_guard<std::mutex> lock(g_mutex);
     if (st->partial_floats < need) {
@@ -924,14 +1017,17 @@ extern "C" int rl_launch_paged_prefill_attention(void* out, int64_t out_row_stri
       st->partials = nullptr;
       st->partial_floats = 0;
       const cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&st->partials), need * sizeof(float));
-      if (e != cudaSuccess) return Fail(static_cast<int>(e), "paged_prefill_attention: %zu MB of scratch: %s", need * 4 >> 20, cudaGetErrorString(e));
+      if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s: %zu MB of scratch: %s", fn, need * 4 >> 20, cudaGetErrorString(e));
       st->partial_floats = need;
     }
+    partials = st->partials;
   }
   Params p;
-  p.n_tiles = n_tiles;
+  p.n_tiles = chunk.Tiles();
   p.split_blocks = split_blocks;
-  p.partials = st->partials;
+  p.partials = partials;
+  p.window = chunk.window;
+  p.sinks = chunk.sinks;
   p.out = static_cast<half*>(out);
   p.out_stride = out_row_stride;
   p.table_row = block_table_row;
@@ -943,31 +1039,89 @@ extern "C" int rl_launch_paged_prefill_attention(void* out, int64_t out_row_stri
   p.scale_log2e = scale * 1.4426950408889634f;
   p.error_flag = st->error_flag;
   const dim3 grid(num_q_heads, static_cast<unsigned>(items));
-  PagedPrefillAttentionKernel<<<grid, kThreads, kSmemBytes, static_cast<cudaStream_t>(stream)>>>(p, q_map, page_map);
-  rc = LaunchStatus("paged_prefill_attention");
+  PagedPrefillAttentionKernel<kWindow><<<grid, kThreads, kSmemBytes, stream>>>(p, q_map, page_map);
+  rc = LaunchStatus(fn);
   if (rc != RL_OK || !any_split) return rc;
-  // Only the chunk's last tiles - the ones with more key blocks than the run length - were cut.
-  int cut_tiles = 0;
-  for (int t = n_tiles - 1; t >= 0; --t) {
-    const int64_t last = std::min<int64_t>(static_cast<int64_t>(chunk_start) + static_cast<int64_t>(t + 1) * kBM, kv_len) - 1;
-    if (static_cast<int>(last / kBN) + 1 <= split_blocks) break;
-    ++cut_tiles;
-  }
   // (a dependent launch whatever the process-wide switch says: the kernel begins with the wait for the stream's
   // previous kernel, which is the one above)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(num_q_heads, cut_tiles, kBM / kCombineRows);
   cfg.blockDim = dim3(kCombineThreads);
-  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, PrefillCombineKernel, p, static_cast<int>(items));
-  if (e != cudaSuccess) return Fail(static_cast<int>(e), "paged_prefill_attention (combine): %s", cudaGetErrorString(e));
-  return LaunchStatus("paged_prefill_attention (combine)");
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, PrefillCombineKernel<kWindow>, p, static_cast<int>(items));
+  if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s (combine): %s", fn, cudaGetErrorString(e));
+  return LaunchStatus(fn);
 }
+
+}  // namespace pfa
+}  // namespace rl
+
+extern "C" int rl_launch_paged_prefill_attention(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                                                 const void* kv_pool_layer, const int32_t* block_table_row,
+                                                 int32_t max_blocks_per_seq, int32_t chunk_start, int32_t chunk_len,
+                                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                 float scale, void* stream) {
+  using namespace rl;
+  using namespace rl::pfa;
+  constexpr const char* fn = "paged_prefill_attention";
+  if (chunk_len <= 0) return RL_OK;
+  const int rc = CheckChunk(fn, out, out_row_stride, q, q_row_stride, kv_pool_layer, block_table_row, max_blocks_per_seq,
+                            chunk_start, chunk_len, num_q_heads, num_kv_heads, head_dim);
+  if (rc != RL_OK) return rc;
+  return LaunchChunk<false>(fn, out, out_row_stride, q, q_row_stride, kv_pool_layer, block_table_row, max_blocks_per_seq,
+                            Chunk{chunk_start, chunk_len, num_q_heads, kWholeWindow, 0}, num_kv_heads, scale, nullptr, 0,
+                            static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int rl_window_prefill_workspace_bytes(int32_t chunk_start, int32_t chunk_len, int32_t num_q_heads,
+                                                 int32_t window, int32_t sinks, size_t* bytes_out) {
+  using namespace rl;
+  using namespace rl::pfa;
+  constexpr const char* fn = "window_prefill_workspace_bytes";
+  if (!bytes_out) return Fail(RL_E_NULL_POINTER, "%s: null pointer", fn);
+  *bytes_out = 0;
+  if (chunk_start < 0 || chunk_len < 0 || num_q_heads < 1 || window < 1 || sinks < 0)
+    return Fail(RL_E_BAD_SHAPE, "%s: chunk_start, chunk_len, sinks >= 0, window and heads >= 1", fn);
+  if (static_cast<int64_t>(chunk_start) + chunk_len > INT32_MAX) return Fail(RL_E_TOO_LARGE, "%s: positions past 2^31", fn);
+  if (chunk_len == 0) return RL_OK;
+  const Chunk chunk = WindowChunk(chunk_start, chunk_len, num_q_heads, window, sinks);
+  int cut_tiles;
+  const int64_t items = CountItems(
+      chunk, g_split_blocks > 0 ? g_split_blocks : ChooseSplitBlocks(chunk, CurrentDeviceFacts().sm_count), &cut_tiles);
+  if (cut_tiles > 0) *bytes_out = static_cast<size_t>(num_q_heads) * items * kPartialFloats * sizeof(float);
+  return RL_OK;
+}
+
+extern "C" int rl_launch_paged_window_prefill_attention(void* out, int64_t out_row_stride, const void* q,
+                                                        int64_t q_row_stride, const void* kv_pool_layer,
+                                                        const int32_t* block_table_row, int32_t max_blocks_per_seq,
+                                                        int32_t chunk_start, int32_t chunk_len, int32_t num_q_heads,
+                                                        int32_t num_kv_heads, int32_t head_dim, float scale,
+                                                        int32_t window, int32_t sinks, void* workspace,
+                                                        size_t workspace_bytes, void* stream) {
+  using namespace rl;
+  using namespace rl::pfa;
+  constexpr const char* fn = "paged_window_prefill_attention";
+  if (chunk_len <= 0) return RL_OK;
+  const int rc = CheckChunk(fn, out, out_row_stride, q, q_row_stride, kv_pool_layer, block_table_row, max_blocks_per_seq,
+                            chunk_start, chunk_len, num_q_heads, num_kv_heads, head_dim);
+  if (rc != RL_OK) return rc;
+  if (num_q_heads / num_kv_heads > 8) return Fail(RL_E_BAD_SHAPE, "%s: at most 8 query heads per KV head", fn);
+  if (window < 1 || sinks < 0) return Fail(RL_E_BAD_SHAPE, "%s: window >= 1 and sinks >= 0", fn);
+  if (max_blocks_per_seq > (1 << 26)) return Fail(RL_E_TOO_LARGE, "%s: at most 2^26 blocks per sequence", fn);
+  if (!(scale > 0.0f) || !(scale * 1.4426950408889634f <= 3.402823466e38f))
+    return Fail(RL_E_BAD_SHAPE, "%s: scale must be positive and finite", fn);
+  if (!Aligned16(workspace)) return Fail(RL_E_BAD_SHAPE, "%s: the workspace must be 16-byte aligned", fn);
+  return LaunchChunk<true>(fn, out, out_row_stride, q, q_row_stride, kv_pool_layer, block_table_row, max_blocks_per_seq,
+                           WindowChunk(chunk_start, chunk_len, num_q_heads, window, sinks), num_kv_heads, scale,
+                           static_cast<float*>(workspace), workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
 extern "C" int rl_prefill_attention_health(int* flag_out) {
   using namespace rl;
   using namespace rl::pfa;
@@ -989,7 +1143,8 @@ extern "C" int rl_prefill_attention_run_length(int32_t chunk_start, int32_t chun
   if (chunk_start < 0 || chunk_len < 1 || num_q_heads < 1 || sm_count < 1)
     return Fail(RL_E_BAD_SHAPE, "rl_prefill_attention_run_length: chunk_start >= 0, chunk_len, heads and SMs >= 1");
   *run_blocks_out = rl::pfa::g_split_blocks > 0 ? rl::pfa::g_split_blocks
-                                                : rl::pfa::ChooseSplitBlocks(chunk_start, chunk_len, num_q_heads, sm_count);
+                                                : rl::pfa::ChooseSplitBlocks(
+                                                      {chunk_start, chunk_len, num_q_heads, rl::pfa::kWholeWindow, 0}, sm_count);
   return RL_OK;
 }
 

@@ -240,51 +240,3 @@ extern "C" int rl_launch_paged_attention_decode_weights(void* out, int64_t out_r
   WeightsKernel<<<dim3(num_seqs, num_kv_heads, 64), 32, 0, s>>>(p);
   return LaunchStatus(fn);
 }
-
-extern "C" int rl_window_prefill_workspace_bytes(int32_t chunk_start, int32_t chunk_len, int32_t num_q_heads,
-                                                 int32_t window, int32_t sinks, size_t* bytes_out) {
-  using namespace rl;
-  if (!bytes_out) return Fail(RL_E_NULL_POINTER, "window_prefill_workspace_bytes: null pointer");
-  *bytes_out = 0;
-  if (chunk_start < 0 || chunk_len < 0 || num_q_heads < 1 || window < 1 || sinks < 0)
-    return Fail(RL_E_BAD_SHAPE, "window_prefill_workspace_bytes: chunk_start, chunk_len, sinks >= 0, window and heads >= 1");
-  return RL_OK;
-}
-
-extern "C" int rl_launch_paged_window_prefill_attention(void* out, int64_t out_row_stride, const void* q,
-                                                        int64_t q_row_stride, const void* kv_pool_layer,
-                                                        const int32_t* block_table_row, int32_t max_blocks_per_seq,
-                                                        int32_t chunk_start, int32_t chunk_len, int32_t num_q_heads,
-                                                        int32_t num_kv_heads, int32_t head_dim, float scale,
-                                                        int32_t window, int32_t sinks, void* workspace,
-                                                        size_t workspace_bytes, void* stream) {
-  using namespace rl;
-  using namespace rl::wattn;
-  constexpr const char* fn = "paged_window_prefill_attention";
-  (void)workspace, (void)workspace_bytes;
-  if (chunk_len <= 0) return RL_OK;
-  int rc = CheckCommon(fn, out, out_row_stride, q, q_row_stride, kv_pool_layer, block_table_row, max_blocks_per_seq,
-                       num_q_heads, num_kv_heads, head_dim, scale);
-  if (rc == RL_OK) rc = CheckWindow(fn, window, sinks);
-  if (rc != RL_OK) return rc;
-  if (chunk_start < 0 || static_cast<int64_t>(chunk_start) + chunk_len > static_cast<int64_t>(max_blocks_per_seq) * kKvBlock)
-    return Fail(RL_E_BAD_SHAPE, "%s: the chunk runs past the block table row", fn);
-  if ((q_row_stride & 7) || (out_row_stride & 7) || !Aligned16(q) || !Aligned16(out))
-    return Fail(RL_E_BAD_SHAPE, "%s: q and out must be 16-byte aligned with row strides in multiples of 8", fn);
-  Params p = {};
-  p.out = static_cast<half*>(out);
-  p.out_stride = out_row_stride;
-  p.q = static_cast<const half*>(q);
-  p.q_stride = q_row_stride;
-  p.pool = static_cast<const half*>(kv_pool_layer);
-  p.tables = block_table_row;
-  p.chunk_start = chunk_start;
-  p.max_blocks = max_blocks_per_seq;
-  p.kv_heads = num_kv_heads;
-  p.group = num_q_heads / num_kv_heads;
-  p.scale_log2e = scale * 1.4426950408889634f;
-  p.window = window;
-  p.sinks = sinks;
-  RowsKernel<<<dim3(chunk_len, num_q_heads), 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return LaunchStatus(fn);
-}
