@@ -47,9 +47,12 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "mma_ptx.cuh"
 
 namespace rl {
 namespace attn {
+
+using namespace rl::mma;
 
 constexpr int kHeadDim = 128;
 constexpr int kGroup = 6;               // query heads per KV head
@@ -196,38 +199,6 @@ __device__ __forceinline__ unsigned long long GlobalTimerNs() {
 #else
 #define RL_STAMP(slot)
 #endif
-__device__ __forceinline__ void Ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void Ldsm4T(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ uint32_t MovmT(uint32_t a) {
-  uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-  return d;
-}
-__device__ __forceinline__ void Mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float Exp2(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t PackHalf2(float lo, float hi) {
-  return AsU32(__floats2half2_rn(lo, hi));
-}
-
 // ------------------------------------------------------- work partition
 
 // First flattened page index of CTA c's share when `total` pages are cut into `ctas` shares.
