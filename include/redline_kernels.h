@@ -424,7 +424,8 @@ int rl_launch_paged_window_prefill_attention(void* out, int64_t out_row_stride, 
  *   any other dst_block_tables: its pages must be apart from every page of the source tables; the source stays as it is.
  * In either case a page belongs to one sequence of the call. new_seq_lens may be seq_lens itself. Slots behind L' in the
  * last destination page keep what they hold. Cached keys keep the rotation of their old positions: the caller goes on
- * counting positions for RoPE apart from cache slots. head_dim a multiple of 8 up to 1024.
+ * counting positions for RoPE apart from cache slots. head_dim a multiple of 8 up to 1024; the pool slice and weights
+ * 16-byte aligned. One call enqueues two kernels.
  */
 int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int32_t* block_tables, int32_t max_blocks_per_seq,
                        const int32_t* dst_block_tables, int32_t dst_max_blocks_per_seq, const int32_t* seq_lens,
