@@ -53,6 +53,29 @@ inline cudaError_t LaunchOverlapped(void (*kernel)(KArgs...), dim3 grid, dim3 bl
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// A dependent launch whatever the switch says, for kernels that touch nothing before griddepcontrol.wait and whose
+// every block executes it: the launch is set up under the tail of the stream's previous kernel, and no order that an
+// ordinary launch would keep is lost. cluster_x > 1: thread-block clusters of that many neighbours along x.
+template <typename... KArgs, typename... Args>
+inline cudaError_t LaunchDependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster_x,
+                                   cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster_x);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster_x > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
 // First statement of a kernel that may be launched by LaunchOverlapped: let the next such launch
 // be set up now, then wait for the previous kernel of the stream (a no-op for ordinary launches).
 __device__ __forceinline__ void DependentLaunchGate() {

@@ -379,31 +379,18 @@ extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int
   const int rc = EnsureReady(fn);
   if (rc != RL_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = LaunchOverlapped(SelectKernel, dim3(num_seqs, num_kv_heads), dim3(kSelectThreads),
-                                   static_cast<size_t>(p.cached_keys) * 4, s, p);
+  cudaError_t e = LaunchDependent(SelectKernel, dim3(num_seqs, num_kv_heads), dim3(kSelectThreads),
+                                  static_cast<size_t>(p.cached_keys) * 4, 1, s, p);
   if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s: %s", fn, cudaGetErrorString(e));
-  // The move is a dependent launch whatever the process-wide switch says: it begins with the wait for the selection.
   const bool in_place = dst_block_tables == block_tables;
   const int64_t most = ((tokens < budget ? tokens : budget) + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
   const int64_t items = static_cast<int64_t>(num_seqs) * num_kv_heads;
   const int64_t fair = (16LL * CurrentDeviceFacts().sm_count + items - 1) / items;
   const int parts = in_place ? kCluster : static_cast<int>(most < fair ? most : fair);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(num_seqs) * parts, num_kv_heads);
-  cfg.blockDim = dim3(kMoveThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kCluster;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = in_place ? 2 : 1;
   const bool plain = head_dim == 128;
-  e = in_place ? (plain ? cudaLaunchKernelEx(&cfg, MoveKernel<true, 32>, p, parts) : cudaLaunchKernelEx(&cfg, MoveKernel<true, 0>, p, parts))
-               : (plain ? cudaLaunchKernelEx(&cfg, MoveKernel<false, 32>, p, parts) : cudaLaunchKernelEx(&cfg, MoveKernel<false, 0>, p, parts));
+  auto kernel = in_place ? (plain ? MoveKernel<true, 32> : MoveKernel<true, 0>) : (plain ? MoveKernel<false, 32> : MoveKernel<false, 0>);
+  e = LaunchDependent(kernel, dim3(static_cast<unsigned>(num_seqs) * parts, num_kv_heads), dim3(kMoveThreads), 0,
+                      in_place ? kCluster : 1, s, p, parts);
   if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s (move): %s", fn, cudaGetErrorString(e));
   return LaunchStatus(fn);
 }

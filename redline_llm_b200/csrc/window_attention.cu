@@ -43,10 +43,12 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 3;
 constexpr int kPageBytes = kKvBlock * kHeadDim * 2;
 constexpr int kStageBytes = 2 * kPageBytes;
-constexpr int kMaxSeqsPerLaunch = 128;
-constexpr int kHeadsPerThread = kMaxGroup / (kThreads / kHeadDim);  // 4: at a merge a thread owns one column of these
-constexpr int kMergeBatch = 4;       // records in flight per thread while merging
+constexpr int kMaxSeqsPerLaunch = 96;
+static_assert(kWarps == kMaxGroup && kHeadDim == 4 * 32, "a fold gives each warp one query head and each lane four columns");
+constexpr int kInlineOthers = 3;     // items over at most this many other CTAs are merged from registers
+constexpr int kMergeBatch = 16;      // longer ones: records in flight per thread
 constexpr int kMinPagesPerCta = kWarps;
+constexpr int kSegmentPages = 12;    // what a second item costs a CTA (fold and hand-over, 2-3 us), in pages
 constexpr int kMaxCtas = 256;
 constexpr int kNewestPageBit = 1 << 30;
 
@@ -56,7 +58,8 @@ constexpr int kOBufOff = kRingBytes;                                   // [warp]
 constexpr int kMlOff = kOBufOff + kWarps * kMaxGroup * kHeadDim * 4;   // m[query][warp], l[query][warp]
 constexpr int kBarOff = kMlOff + 2 * kMaxGroup * kWarps * 4;
 constexpr int kPrefixOff = kBarOff + kWarps * kStages * 8;
-constexpr int kSkipOff = kPrefixOff + (kMaxSeqsPerLaunch + 4) * 4;
+constexpr int kChunkOff = kPrefixOff + (kMaxSeqsPerLaunch + 4) * 4;
+constexpr int kSkipOff = kChunkOff + (kMaxSeqsPerLaunch + 4) * 4;
 constexpr int kSmemBytes = kSkipOff + kMaxSeqsPerLaunch * 4 + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "window attention shared memory exceeds the 227 KB per-CTA limit");
 
@@ -85,9 +88,10 @@ struct Params {
   int* meta;
   float* records;
   float2* stats;       // [sequence][query head]: maximum (log2 domain), 1 / sum
-  float* scores;       // [sequence][KV head][page][16][score_pitch], log2 domain
-  int score_pitch;
+  float* scores;       // [sequence][KV head][page][query of the group][16], log2 domain
   float* weights;
+  bool wide_out;       // out rows are 8-byte aligned
+  bool run_ahead;      // the overlap option: lengths, tables and all but the newest pages may be read before the wait
 };
 
 // A page's K tile and V tile of one KV head, 8 KiB, in one copy into this CTA's shared memory (no multicast).
@@ -136,55 +140,105 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   float* mbuf = reinterpret_cast<float*>(smem + kMlOff);
   float* lbuf = mbuf + kMaxGroup * kWarps;
   int* prefix = reinterpret_cast<int*>(smem + kPrefixOff);
+  int* chunk_prefix = reinterpret_cast<int*>(smem + kChunkOff);
   int* skip = reinterpret_cast<int*>(smem + kSkipOff);   // pages between a sequence's sinks and its window
-  __shared__ int warp_total[kMaxSeqsPerLaunch / 32];
+  __shared__ int warp_total[kMaxSeqsPerLaunch / 32], warp_live[kMaxSeqsPerLaunch / 32], warp_most[kMaxSeqsPerLaunch / 32], warp_chunks[kMaxSeqsPerLaunch / 32];
   __shared__ bool merge_here, others_done;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, tig = lane & 3;
   const int heads = p.kv_heads;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!kScores) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == kThreads - 1) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tile_map) : "memory");
     for (int b = 0; b < kStages * kWarps; ++b) MbarInit(SmemAddr(smem + kBarOff) + b * 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  {  // page prefix over the sequences, one per thread; every CTA works out the same table
-    int n = 0, incl = 0;
-    if (tid < kMaxSeqsPerLaunch) {
-      const int len = tid < p.num_seqs ? min(p.seq_lens[tid], p.max_blocks * kKvBlock) : 0;
-      if (len > 0) {
-        const int pages = (len + kKvBlock - 1) >> kKvBlockShift;
-        const int window_page = max(0, len - p.window) >> kKvBlockShift;
-        const int gap = max(0, window_page - p.sink_pages);
-        n = pages - gap;
-        skip[tid] = gap;
-      }
-      incl = n;
+  if (!p.run_ahead) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // Page prefix over the sequences, one per thread; every CTA works out the same table.
+  int my_pages = 0;
+  auto scan_sequences = [&](int value, int* totals) {   // inclusive scan over the first kMaxSeqsPerLaunch threads
+    int incl = value;
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += v;
-      }
-      if (lane == 31) warp_total[warp] = incl;
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += v;
     }
+    if (lane == 31 && tid < kMaxSeqsPerLaunch) totals[warp] = incl;
     __syncthreads();
-    if (tid < kMaxSeqsPerLaunch) {
-      for (int w = 0; w < warp; ++w) incl += warp_total[w];
-      prefix[tid + 1] = incl;
-      if (tid == 0) prefix[0] = 0;
+    for (int w = 0; w < warp && w < kMaxSeqsPerLaunch / 32; ++w) incl += totals[w];
+    return incl;
+  };
+  if (tid < p.num_seqs) {
+    const int len = min(p.seq_lens[tid], p.max_blocks * kKvBlock);
+    if (len > 0) {
+      const int window_page = max(0, len - p.window) >> kKvBlockShift;
+      const int gap = max(0, window_page - p.sink_pages);
+      my_pages = ((len + kKvBlock - 1) >> kKvBlockShift) - gap;
+      skip[tid] = gap;
     }
+  }
+  {
+    const unsigned live = __ballot_sync(0xffffffffu, my_pages > 0);
+    const int most = __reduce_max_sync(0xffffffffu, my_pages);
+    if (lane == 0 && tid < kMaxSeqsPerLaunch) {
+      warp_live[warp] = __popc(live);
+      warp_most[warp] = most;
+    }
+    const int incl = scan_sequences(my_pages, warp_total);
+    if (tid < kMaxSeqsPerLaunch) prefix[tid + 1] = incl;
+    if (tid == 0) prefix[0] = chunk_prefix[0] = 0;
     __syncthreads();
   }
   const long long total = static_cast<long long>(heads) * prefix[p.num_seqs];
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(1LL, total / kMinPagesPerCta)));
-  const int cta = blockIdx.x;
-  if (total == 0 || cta >= ctas) {
+  if (total == 0) {
     asm volatile("griddepcontrol.wait;" ::: "memory");   // this grid never completes ahead of the one before it
     return;
   }
-  const long long share_begin = ShareBegin(cta, total, ctas), share_end = ShareBegin(cta + 1, total, ctas);
+  int items = 0, most_pages = 0;
+  for (int w = 0; w < kMaxSeqsPerLaunch / 32; ++w) {
+    items += heads * warp_live[w];
+    most_pages = max(most_pages, warp_most[w]);
+  }
+  const int cta = blockIdx.x;
+  // How the pages are cut: equal shares of the flattened list, whatever items they meet - or, where there are few items,
+  // each item in equal chunks with a CTA each. The longest chunk is longer than a share (74 pages against 62 where 24 items
+  // of 380 meet 148 CTAs), but no CTA meets a second item, whose fold and hand-over cost it as much as kSegmentPages pages.
+  // (Both measured, shares and chunks: 7 sequences of 3-2500 tokens, 28 items, 21.3 and 10.8 us; 8 x 4096, 16 items, 21.2
+  // and 14.4 us; 64 x 1024-1280, 128 items, stay with shares.)
+  int longest = 0;
+  bool chunked = false;
+  if (items < static_cast<int>(gridDim.x)) {
+    const int spare = static_cast<int>(gridDim.x) - items;
+    const long long fit = (total + spare - 1) / spare;   // sum of ceil(pages / fit) <= total / fit + items <= the grid
+    longest = static_cast<int>(max(min(fit, static_cast<long long>(most_pages)), static_cast<long long>(kMinPagesPerCta)));
+    chunked = longest <= total / static_cast<int>(gridDim.x) + kSegmentPages;
+  }
+  long long share_begin, share_end;
+  int ctas, chunk_first = 0, chunk_last = 0;   // (chunked) the CTAs of this CTA's item
+  if (chunked) {
+    const int chunks = my_pages > 0 ? (my_pages + longest - 1) / longest : 0;
+    const int incl = scan_sequences(chunks, warp_chunks);
+    if (tid < kMaxSeqsPerLaunch) chunk_prefix[tid + 1] = incl;
+    __syncthreads();
+    ctas = heads * chunk_prefix[p.num_seqs];   // <= total / longest + items <= gridDim.x
+    const Cursor c = Locate(cta < ctas ? cta : 0, chunk_prefix, p.num_seqs, heads);   // entry = chunk, entries = chunks
+    const long long pages = prefix[c.seq + 1] - prefix[c.seq];
+    const long long item = static_cast<long long>(heads) * prefix[c.seq] + c.head * pages;
+    share_begin = item + c.entry * pages / c.entries;
+    share_end = item + (c.entry + 1) * pages / c.entries;
+    chunk_first = cta - c.entry;
+    chunk_last = chunk_first + c.entries - 1;
+  } else {
+    ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(1LL, total / kMinPagesPerCta)));
+    share_begin = ShareBegin(cta, total, ctas);
+    share_end = ShareBegin(cta + 1, total, ctas);
+  }
+  if (cta >= ctas) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
 
   // ---- this warp's pages: share-relative indices warp, warp + 8, ...
   const int share_len = static_cast<int>(share_end - share_begin);
@@ -222,6 +276,9 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
     if (!(tile & kNewestPageBit)) request(i, tile);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // The kernel that adds the weights up reads the old ones ahead of its own wait: it may start only now that whatever
+  // wrote them before this grid is done.
+  if (kScores) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 #pragma unroll 1
   for (int i = 0; i < first; ++i) {
     const int tile = __shfl_sync(0xffffffffu, tiles_cur, i);
@@ -274,13 +331,17 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
     }
     const bool whole = seg_begin == item_begin && seg_end == item_end;
     int c_first = cta, c_last = cta;
-    if (!whole) {
+    if (chunked) {
+      c_first = chunk_first;
+      c_last = chunk_last;
+    } else if (!whole) {
       if (item_begin < share_begin) c_first = ShareOf(item_begin, total, ctas);
       if (item_end > share_end) c_last = ShareOf(item_end - 1, total, ctas);
     }
     const int others = c_last - c_first;
-    const bool may_read_inline = !whole && others < kMergeBatch;
+    const bool may_read_inline = !whole && others <= kInlineOthers;
     int* ticket = p.meta + kTicketOff + c_first;
+    float* seg_scores = kScores ? p.scores + (static_cast<int64_t>(sc.seq) * heads + sc.head) * p.max_blocks * (kKvBlock * p.group) : nullptr;
     int seen = -1;   // thread 0: how many of the others had published when it looked
 
     float o[8][4];
@@ -317,11 +378,16 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[i] = (s[i] + s2[i]) * p.scale_log2e;
-        if (kScores && 2 * tig < p.score_pitch) {
-          float* row = p.scores + ((static_cast<int64_t>(sc.seq) * heads + sc.head) * p.max_blocks + page) * (kKvBlock * p.score_pitch) +
-                       g * p.score_pitch + 2 * tig;
-          *reinterpret_cast<float2*>(row) = make_float2(s[0], s[1]);
-          *reinterpret_cast<float2*>(row + 8 * p.score_pitch) = make_float2(s[2], s[3]);
+        if (kScores) {   // [query][token]: the eight lanes of a query fill whole sectors
+          float* dst = seg_scores + static_cast<int64_t>(page) * (kKvBlock * p.group) + 2 * tig * kKvBlock + g;
+          if (2 * tig < p.group) {
+            __stcg(dst, s[0]);
+            __stcg(dst + 8, s[2]);
+          }
+          if (2 * tig + 1 < p.group) {
+            __stcg(dst + kKvBlock, s[1]);
+            __stcg(dst + kKvBlock + 8, s[3]);
+          }
         }
         auto visible = [&](int i) { return i < end && (i < sink || i >= win); };
         if (!full) {
@@ -410,106 +476,122 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
       }
     }
     __syncthreads();
-    const int d = tid & (kHeadDim - 1), q0 = (tid >> 7) * kHeadsPerThread;   // this thread: column d of queries q0 .. q0 + 3
-    float rm[kMergeBatch][kHeadsPerThread], rl_[kMergeBatch][kHeadsPerThread], ro[kMergeBatch][kHeadsPerThread];
-    auto load_records = [&](int c0) {
+    // From here on warp h has query head h of the group, lane i its columns 4i .. 4i + 3.
+    const bool has_head = warp < p.group;
+    const int d = 4 * lane;
+    // a contributor's record 0 is of an item that began before its share, record 1 of one that begins in it
+    auto record = [&](int c) { return p.records + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kRecordFloats; };
+    float om[kInlineOthers], ol[kInlineOthers];
+    float4 oo[kInlineOthers];
+    auto load_others = [&]() {   // the other contributors' records, in CTA order
 #pragma unroll
-      for (int j = 0; j < kMergeBatch; ++j) {
-        const int c = c0 + j;
-        if (c <= c_last && c != cta) {
-          // a contributor's record 0 is of an item that began before its share, record 1 of one that begins in it
-          const float* r = p.records + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kRecordFloats;
-#pragma unroll
-          for (int qi = 0; qi < kHeadsPerThread; ++qi) {
-            if (q0 + qi < p.group) {
-              ro[j][qi] = __ldcg(r + (q0 + qi) * kHeadDim + d);
-              rm[j][qi] = __ldcg(r + kMaxGroup * kHeadDim + q0 + qi);
-              rl_[j][qi] = __ldcg(r + kMaxGroup * kHeadDim + kMaxGroup + q0 + qi);
-            }
-          }
+      for (int j = 0; j < kInlineOthers; ++j) {
+        if (j < others && has_head) {
+          const float* r = record(c_first + j + (c_first + j >= cta ? 1 : 0));
+          om[j] = __ldcg(r + kMaxGroup * kHeadDim + warp);
+          ol[j] = __ldcg(r + kMaxGroup * kHeadDim + kMaxGroup + warp);
+          oo[j] = __ldcg(reinterpret_cast<const float4*>(r + warp * kHeadDim + d));
         }
       }
     };
     const bool fast = !whole && others_done;
-    if (fast) load_records(c_first);
-    float acc[kHeadsPerThread], mx[kHeadsPerThread], den[kHeadsPerThread];
-#pragma unroll
-    for (int qi = 0; qi < kHeadsPerThread; ++qi) {
-      const int q = q0 + qi;
-      acc[qi] = den[qi] = 0.0f;
-      mx[qi] = -INFINITY;
-      if (q < p.group) {
-        float mw[kWarps], lw[kWarps];
-#pragma unroll
-        for (int i = 0; i < kWarps / 4; ++i) {
-          const float4 m4 = reinterpret_cast<const float4*>(mbuf + q * kWarps)[i];
-          const float4 l4 = reinterpret_cast<const float4*>(lbuf + q * kWarps)[i];
-          mw[4 * i] = m4.x, mw[4 * i + 1] = m4.y, mw[4 * i + 2] = m4.z, mw[4 * i + 3] = m4.w;
-          lw[4 * i] = l4.x, lw[4 * i + 1] = l4.y, lw[4 * i + 2] = l4.z, lw[4 * i + 3] = l4.w;
-        }
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) mx[qi] = fmaxf(mx[qi], mw[w]);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float f = Exp2(mw[w] - mx[qi]);   // 0 for a warp that saw no page
-          acc[qi] = fmaf(f, obuf[(w * kMaxGroup + q) * kHeadDim + (d ^ ((q >> 1) * 8))], acc[qi]);
-          den[qi] = fmaf(f, lw[w], den[qi]);
-        }
-      }
-    }
-    auto write_item = [&](const float (&a)[kHeadsPerThread], const float (&m)[kHeadsPerThread], const float (&l)[kHeadsPerThread]) {
-#pragma unroll
-      for (int qi = 0; qi < kHeadsPerThread; ++qi) {
-        if (q0 + qi < p.group) {
-          const int qh = sc.head * p.group + q0 + qi;
-          p.out[static_cast<int64_t>(sc.seq) * p.out_stride + static_cast<int64_t>(qh) * kHeadDim + d] = __float2half_rn(a[qi] / l[qi]);
-          if (kScores && d == 0) p.stats[static_cast<int64_t>(sc.seq) * heads * p.group + qh] = make_float2(m[qi], 1.0f / l[qi]);
-        }
-      }
+    if (fast) load_others();
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float mx = -INFINITY, den = 0.0f;
+    auto add_part = [](float f, const float4& v, float l, float4& a, float& sum) {
+      a.x = fmaf(f, v.x, a.x);
+      a.y = fmaf(f, v.y, a.y);
+      a.z = fmaf(f, v.z, a.z);
+      a.w = fmaf(f, v.w, a.w);
+      sum = fmaf(f, l, sum);
     };
-    // The item from every contributor's record, in CTA order (this CTA's own from its registers).
-    auto merge = [&](bool first_loaded) {
-      float a[kHeadsPerThread], m[kHeadsPerThread], l[kHeadsPerThread];
+    if (has_head) {
+      float mw[kWarps];
 #pragma unroll
-      for (int qi = 0; qi < kHeadsPerThread; ++qi) a[qi] = l[qi] = 0.0f, m[qi] = -INFINITY;
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, mw[w] = mbuf[warp * kWarps + w]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)   // a factor of 0 for a warp that saw no page
+        add_part(Exp2(mw[w] - mx), *reinterpret_cast<const float4*>(obuf + (w * kMaxGroup + warp) * kHeadDim + (d ^ ((warp >> 1) * 8))),
+                 lbuf[warp * kWarps + w], acc, den);
+    }
+    auto write_item = [&](const float4& a, float m, float l) {
+      if (!has_head) return;
+      const int qh = sc.head * p.group + warp;
+      half* dst = p.out + static_cast<int64_t>(sc.seq) * p.out_stride + static_cast<int64_t>(qh) * kHeadDim + d;
+      const half2 lo = __floats2half2_rn(a.x / l, a.y / l), hi = __floats2half2_rn(a.z / l, a.w / l);
+      if (p.wide_out) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(AsU32(lo), AsU32(hi));
+      } else {
+        dst[0] = __low2half(lo);
+        dst[1] = __high2half(lo);
+        dst[2] = __low2half(hi);
+        dst[3] = __high2half(hi);
+      }
+      if (kScores && lane == 0) p.stats[static_cast<int64_t>(sc.seq) * heads * p.group + qh] = make_float2(m, 1.0f / l);
+    };
+    // Few contributors: from registers, in CTA order with one common maximum, whoever does it.
+    auto merge_few = [&]() {
+      float m = mx;
+#pragma unroll
+      for (int j = 0; j < kInlineOthers; ++j)
+        if (j < others) m = fmaxf(m, om[j]);
+      float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float l = 0.0f;
+#pragma unroll
+      for (int j = 0; j <= kInlineOthers; ++j) {   // own record in its place among the others
+        if (c_first + j == cta) add_part(Exp2(mx - m), acc, den, a, l);
+        if (j < kInlineOthers && j < others) add_part(Exp2(om[j] - m), oo[j], ol[j], a, l);
+      }
+      write_item(a, m, l);
+    };
+    // Many: the factors of all records first (in the fold's buffer, which is free), then the records themselves,
+    // kMergeBatch in flight - one L2 latency per batch on the path that the whole grid waits for.
+    auto merge_many = [&]() {
+      if (!has_head) return;
+      float* factor = obuf + warp * kMaxCtas;
+      float m = -INFINITY;
+      for (int c = c_first + lane; c <= c_last; c += 32) {
+        const float mc = __ldcg(record(c) + kMaxGroup * kHeadDim + warp);
+        factor[c - c_first] = mc;
+        m = fmaxf(m, mc);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+      float l = 0.0f;
+      for (int c = c_first + lane; c <= c_last; c += 32) {
+        const float f = Exp2(factor[c - c_first] - m);
+        factor[c - c_first] = f;
+        l = fmaf(f, __ldcg(record(c) + kMaxGroup * kHeadDim + kMaxGroup + warp), l);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+      __syncwarp();
+      float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
       for (int c0 = c_first; c0 <= c_last; c0 += kMergeBatch) {
-        if (!first_loaded) load_records(c0);
-        first_loaded = false;
+        float4 v[kMergeBatch];
 #pragma unroll
-        for (int j = 0; j < kMergeBatch; ++j) {
-          if (c0 + j <= c_last) {
-            const bool mine = c0 + j == cta;
+        for (int j = 0; j < kMergeBatch; ++j)
+          if (c0 + j <= c_last) v[j] = __ldcg(reinterpret_cast<const float4*>(record(c0 + j) + warp * kHeadDim + d));
+        float unused = 0.0f;
 #pragma unroll
-            for (int qi = 0; qi < kHeadsPerThread; ++qi) {
-              if (q0 + qi < p.group) {
-                const float mc = mine ? mx[qi] : rm[j][qi], lc = mine ? den[qi] : rl_[j][qi], oc = mine ? acc[qi] : ro[j][qi];
-                const float n = fmaxf(m[qi], mc), keep = Exp2(m[qi] - n), add = Exp2(mc - n);
-                a[qi] = fmaf(add, oc, a[qi] * keep);
-                l[qi] = fmaf(add, lc, l[qi] * keep);
-                m[qi] = n;
-              }
-            }
-          }
-        }
+        for (int j = 0; j < kMergeBatch; ++j)
+          if (c0 + j <= c_last) add_part(factor[c0 + j - c_first], v[j], 0.0f, a, unused);
       }
       write_item(a, m, l);
     };
     if (whole) {
       write_item(acc, mx, den);
     } else if (fast) {
-      merge(true);
+      merge_few();
       if (tid == 0) *ticket = 0;   // everyone had arrived: ready for the next launch
     } else {
       float* rec = p.records + (static_cast<size_t>(cta) * 2 + (item_begin < share_begin ? 0 : 1)) * kRecordFloats;
-#pragma unroll
-      for (int qi = 0; qi < kHeadsPerThread; ++qi) {
-        if (q0 + qi < p.group) {
-          rec[(q0 + qi) * kHeadDim + d] = acc[qi];
-          if (d == 0) {
-            rec[kMaxGroup * kHeadDim + q0 + qi] = mx[qi];
-            rec[kMaxGroup * kHeadDim + kMaxGroup + q0 + qi] = den[qi];
-          }
+      if (has_head) {
+        *reinterpret_cast<float4*>(rec + warp * kHeadDim + d) = acc;
+        if (lane == 0) {
+          rec[kMaxGroup * kHeadDim + warp] = mx;
+          rec[kMaxGroup * kHeadDim + kMaxGroup + warp] = den;
         }
       }
       __syncthreads();
@@ -521,7 +603,12 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
       __syncthreads();
       if (merge_here) {
         __threadfence();
-        merge(false);
+        if (others <= kInlineOthers) {
+          load_others();
+          merge_few();
+        } else {
+          merge_many();
+        }
       }
     }
     __syncthreads();   // obuf and the flags are free for the next segment
@@ -533,29 +620,57 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
 }
 
 // Second kernel of the weights launcher: per cached token and KV head, the sum over the group of
-// exp2(score - maximum) / sum, added to the token's weight. One thread per (head, page, slot) of a sequence; a token's
-// scores of the group lie side by side, so a warp reads and writes whole lines.
-__global__ void __launch_bounds__(256) AccumulateKernel(const Params p, int parts) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+// exp2(score - maximum) / sum, added to the token's weight. One thread per token, 16 neighbours to a page: scores of a
+// query, and weights, are read and written in whole lines. What the kernel before it does not write - lengths, table,
+// old weights - is read ahead of the wait for it.
+constexpr int kAccumulateThreads = 256;
+constexpr int kTokensPerThread = 2;   // in flight together: the kernel is a chain of loads, not a stream
+constexpr int kAccumulateTokens = kAccumulateThreads * kTokensPerThread;
+__global__ void __launch_bounds__(kAccumulateThreads) AccumulateKernel(const Params p, int parts) {
+  const int part = blockIdx.x % parts, head = blockIdx.y;
   const int64_t seq = blockIdx.x / parts;
-  const int part = blockIdx.x % parts;
   const int len = min(p.seq_lens[seq], p.max_blocks * kKvBlock);
-  if (len <= 0) return;
-  const int slots = ((len + kKvBlock - 1) >> kKvBlockShift) * kKvBlock;
   const int32_t* table = p.tables + seq * p.max_blocks;
-  for (int64_t i = part * 256 + threadIdx.x; i < static_cast<int64_t>(slots) * p.kv_heads; i += static_cast<int64_t>(parts) * 256) {
-    const int head = static_cast<int>(i / slots), t = static_cast<int>(i - static_cast<int64_t>(head) * slots);
-    if (t >= len) continue;
-    const float2* st = p.stats + (seq * p.kv_heads + head) * p.group;
-    const float* s = p.scores + ((seq * p.kv_heads + head) * p.max_blocks * kKvBlock + t) * p.score_pitch;
-    float sum = 0.0f;
-    for (int q = 0; q < p.group; ++q) {
-      const float2 ml = __ldcg(st + q);
-      sum = fmaf(Exp2(__ldcg(s + q) - ml.x), ml.y, sum);
+  const float2* st = p.stats + (seq * p.kv_heads + head) * p.group;
+  const float* scores = p.scores + (seq * p.kv_heads + head) * p.max_blocks * (kKvBlock * p.group);
+  bool waited = false;
+  float2 ml[kMaxGroup];
+#pragma unroll 1
+  for (int64_t t0 = part * kAccumulateTokens; t0 < len; t0 += static_cast<int64_t>(parts) * kAccumulateTokens) {
+    float* w[kTokensPerThread];
+    float old[kTokensPerThread];
+#pragma unroll
+    for (int k = 0; k < kTokensPerThread; ++k) {
+      const int64_t t = t0 + k * kAccumulateThreads + threadIdx.x;
+      w[k] = t < len ? p.weights + (static_cast<int64_t>(table[t >> kKvBlockShift]) * p.kv_heads + head) * kKvBlock + (t & (kKvBlock - 1)) : nullptr;
     }
-    float* w = p.weights + (static_cast<int64_t>(table[t >> kKvBlockShift]) * p.kv_heads + head) * kKvBlock + (t & (kKvBlock - 1));
-    *w = t == len - 1 ? sum : *w + sum;
+#pragma unroll
+    for (int k = 0; k < kTokensPerThread; ++k)
+      old[k] = w[k] && t0 + k * kAccumulateThreads + threadIdx.x != len - 1 ? *w[k] : 0.0f;
+    if (!waited) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      waited = true;
+#pragma unroll
+      for (int q = 0; q < kMaxGroup; ++q) ml[q] = q < p.group ? __ldcg(st + q) : make_float2(0.0f, 0.0f);
+    }
+    float x[kTokensPerThread][kMaxGroup];
+#pragma unroll
+    for (int k = 0; k < kTokensPerThread; ++k) {
+      const int64_t t = t0 + k * kAccumulateThreads + threadIdx.x;
+      const float* s = scores + (t >> kKvBlockShift) * (kKvBlock * p.group) + (t & (kKvBlock - 1));
+#pragma unroll
+      for (int q = 0; q < kMaxGroup; ++q) x[k][q] = w[k] && q < p.group ? __ldcg(s + q * kKvBlock) : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < kTokensPerThread; ++k) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kMaxGroup; ++q)
+        if (q < p.group) sum = fmaf(Exp2(x[k][q] - ml[q].x), ml[q].y, sum);
+      if (w[k]) *w[k] = old[k] + sum;
+    }
   }
+  if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ----------------------------------------------------------- host side
@@ -609,13 +724,11 @@ bool ShapeOk(int max_blocks, int q_heads, int kv_heads) {
   return max_blocks >= 1 && max_blocks <= kMaxBlocks && kv_heads >= 1 && kv_heads <= kMaxKvHeads && q_heads >= kv_heads &&
          q_heads % kv_heads == 0 && q_heads / kv_heads <= kMaxGroup;
 }
-int ScorePitch(int group) { return (group + 1) & ~1; }
 size_t StatsBytes(int64_t num_seqs, int q_heads) { return (static_cast<size_t>(num_seqs) * q_heads * sizeof(float2) + 255) & ~static_cast<size_t>(255); }
 size_t Workspace(int64_t num_seqs, int max_blocks, int q_heads, int kv_heads, bool weights) {
   size_t bytes = kMetaBytes + kRecordBytes;
   if (weights)
-    bytes += StatsBytes(num_seqs, q_heads) + static_cast<size_t>(num_seqs) * kv_heads * max_blocks * kKvBlock *
-                                                 ScorePitch(q_heads / kv_heads) * sizeof(float);
+    bytes += StatsBytes(num_seqs, q_heads) + static_cast<size_t>(num_seqs) * q_heads * max_blocks * kKvBlock * sizeof(float);
   return bytes;
 }
 
@@ -682,14 +795,15 @@ int Launch(const Call& c) {
   p.records = reinterpret_cast<float*>(ws + kMetaBytes);
   float2* stats = reinterpret_cast<float2*>(ws + kMetaBytes + kRecordBytes);
   float* scores = reinterpret_cast<float*>(ws + kMetaBytes + kRecordBytes + StatsBytes(c.num_seqs, c.q_heads));
-  p.score_pitch = ScorePitch(p.group);
+  p.run_ahead = g_launch_overlap;
+  p.wide_out = (reinterpret_cast<uintptr_t>(c.out) & 7) == 0 && (c.out_row_stride & 3) == 0;
   // No more CTAs than shares of kMinPagesPerCta pages can exist: a row's list is at most this long.
   const int64_t list = p.sink_pages + ((p.window + kKvBlock - 2) >> kKvBlockShift) + 1;
   const int64_t pages = list < c.max_blocks ? list : c.max_blocks;
   if (pages * kMaxSeqsPerLaunch > INT32_MAX && pages * c.num_seqs > INT32_MAX)
     return Fail(RL_E_TOO_LARGE, "%s: more than 2^31 pages in one call", c.fn);
   const int sms = CurrentDeviceFacts().sm_count < kMaxCtas ? CurrentDeviceFacts().sm_count : kMaxCtas;
-  const int64_t row = static_cast<int64_t>(c.kv_heads) * c.max_blocks * kKvBlock * p.score_pitch;
+  const int64_t row = static_cast<int64_t>(c.q_heads) * c.max_blocks * kKvBlock;
   for (int first = 0; first < c.num_seqs; first += kMaxSeqsPerLaunch) {
     const int n = c.num_seqs - first < kMaxSeqsPerLaunch ? c.num_seqs - first : kMaxSeqsPerLaunch;
     p.out = static_cast<half*>(c.out) + first * c.out_row_stride;
@@ -699,9 +813,9 @@ int Launch(const Call& c) {
     p.num_seqs = n;
     p.stats = stats + static_cast<int64_t>(first) * c.q_heads;
     p.scores = scores + first * row;
-    const int64_t shares = (n * c.kv_heads * pages) / kMinPagesPerCta;
+    const int64_t shares = static_cast<int64_t>(n) * c.kv_heads * ((pages + kMinPagesPerCta - 1) / kMinPagesPerCta);
     const int grid = static_cast<int>(shares < 1 ? 1 : shares < sms ? shares : sms);
-    const cudaError_t e = LaunchOverlapped(DecodeKernel<kScores>, dim3(grid), dim3(kThreads), kSmemBytes, c.stream, p, tile_map);
+    const cudaError_t e = LaunchDependent(DecodeKernel<kScores>, dim3(grid), dim3(kThreads), kSmemBytes, 1, c.stream, p, tile_map);
     if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s: %s", c.fn, cudaGetErrorString(e));
   }
   if (kScores) {
@@ -710,20 +824,13 @@ int Launch(const Call& c) {
     p.stats = stats;
     p.scores = scores;
     p.weights = c.weights;
-    // enough CTAs per sequence for its longest possible cache, but no more in all than fill the machine a few times
-    const int64_t most = (static_cast<int64_t>(c.max_blocks) * kKvBlock * c.kv_heads + 255) / 256;
-    const int64_t fair = (8LL * sms + c.num_seqs - 1) / c.num_seqs;
+    // enough CTAs per item for its longest possible cache, but no more in all than fill the machine
+    const int64_t most = (static_cast<int64_t>(c.max_blocks) * kKvBlock + kAccumulateTokens - 1) / kAccumulateTokens;
+    const int64_t items = static_cast<int64_t>(c.num_seqs) * c.kv_heads;
+    const int64_t fair = (8LL * sms + items - 1) / items;
     const int parts = static_cast<int>(most < fair ? most : fair);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(c.num_seqs) * parts);
-    cfg.blockDim = dim3(256);
-    cfg.stream = c.stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;   // it begins with the wait for the kernel above
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, AccumulateKernel, p, parts);
+    const cudaError_t e = LaunchDependent(AccumulateKernel, dim3(static_cast<unsigned>(c.num_seqs) * parts, c.kv_heads),
+                                          dim3(kAccumulateThreads), 0, 1, c.stream, p, parts);
     if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s (weights): %s", c.fn, cudaGetErrorString(e));
   }
   return LaunchStatus(c.fn);
