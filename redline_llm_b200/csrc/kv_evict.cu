@@ -6,12 +6,12 @@
 //
 // Two kernels. What bounds them: the selection is a chain of short dependent passes (latency), the move is a copy of
 // the kept rows (HBM).
-//  * Select, one CTA per (sequence, KV head): weights become integers that compare the same way and stay in shared
-//    memory; a radix select of three digits (11, 11, 10 bits) finds the weight of the last kept token - a histogram per
-//    digit, its suffix sums over the block, and on to the digit below among the keys that share the prefix; then one
-//    ordered sweep writes the kept positions, each warp a stretch of the sequence, ballots giving the ranks.
+//  * Select, one CTA or a cluster of them per (sequence, KV head): weights become integers that compare the same way and stay in shared
+//    memory; a histogram over their range and its suffix sums name the bin of the last kept token, whose keys leave the
+//    crowd - one per thread - and are divided further until the last few are ranked against one another; then an ordered
+//    sweep writes the kept positions, each warp a stretch of the sequence, warp scans giving the ranks.
 //  * Move, 32 rows per warp: a lane looks up one row's source and destination, then the warp copies the rows 16 bytes a
-//    lane, sixteen rows in flight. In place a cluster of eight CTAs walks a (sequence, head) in cache order, every row of a round
+//    lane, eight rows in flight. In place a cluster of eight CTAs walks a (sequence, head) in cache order, every row of a round
 //    read before any of it is written: a row never moves to a higher slot, so what a round overwrites was read in it or
 //    before it.
 #include <mutex>
@@ -52,73 +52,182 @@ __device__ __forceinline__ int CachedTokens(const Params& p, int seq) {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWarps = kSelectThreads / 32;
-constexpr int kBins = 2048;
-constexpr int kMaxCachedKeys = 48 * 1024;   // 192 KB
+constexpr int kMaxSelectCluster = 8;
+constexpr int kBinBits = 11, kBins = 1 << kBinBits;
+constexpr int kListed = 1024;      // candidates of a bin that are taken out of the crowd: one per thread
+constexpr int kRanked = 64;        // of those, as many as are simply ranked against one another
+constexpr int kLoadAhead = 8;      // quads of weights a thread has in flight
+constexpr int kMaxCachedKeys = 45 * 1024;   // 180 KB
+static_assert(kBins == 2 * kSelectThreads && kListed <= kSelectThreads, "two bins per thread, a thread per listed key");
 
-__global__ void __launch_bounds__(kSelectThreads) SelectKernel(const Params p) {
+// What the CTAs of a cluster tell one another.
+struct Shared {
+  int bins[kBins];
+  uint32_t list[kListed];
+  uint32_t lo, hi;       // range of this CTA's keys
+  int listed;            // keys in its list
+  int sure, equal;       // its tokens above the threshold (or kept in any case), and at it
+};
+
+__device__ __forceinline__ void ClusterBarrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A 32-bit word of the same variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t LoadPeer(const void* mine, int rank) {
+  uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(mine)), v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ int2 LoadPeer2(const int* mine, int rank) {   // two words, 8-byte aligned
+  uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
+  int2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// Grid: (sequences * cluster, KV heads). CTA `rank` of an item's cluster has every quad of tokens of its slice.
+__global__ void __launch_bounds__(kSelectThreads, 1) SelectKernel(const Params p, int cluster) {
   extern __shared__ __align__(16) uint32_t keys[];
-  __shared__ int bins[kBins];
+  __shared__ __align__(16) Shared sh;
+  __shared__ __align__(16) uint32_t crowd[kListed + 4];
+  __shared__ int local_bins[kBins];
   __shared__ int warp_sum[kSelectWarps], warp_equal[kSelectWarps];
+  __shared__ uint32_t warp_lo[kSelectWarps], warp_hi[kSelectWarps], found_key;
   __shared__ int found_bin, found_above, found_count;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int seq = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int seq = blockIdx.x / cluster, rank = blockIdx.x % cluster, head = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int len = CachedTokens(p, seq);
   const int n = min(len, p.budget);
   const int32_t* table = p.tables + static_cast<int64_t>(seq) * p.max_blocks;
   int32_t* kept = p.kept + (static_cast<int64_t>(seq) * p.kv_heads + head) * p.budget;
-  for (int j = n + tid; j < p.budget; j += kSelectThreads) kept[j] = -1;
-  if (len <= p.budget) {
-    for (int j = tid; j < n; j += kSelectThreads) kept[j] = j;
+  for (int j = n + rank * kSelectThreads + tid; j < p.budget; j += cluster * kSelectThreads) kept[j] = -1;
+  if (len <= p.budget) {   // (the same for the whole cluster)
+    for (int j = rank * kSelectThreads + tid; j < n; j += cluster * kSelectThreads) kept[j] = j;
     return;
   }
-  // candidates are tokens [a, b); their keys are handled four at a time from a4 on (four neighbours share a page)
-  const int a = p.sinks, b = len - p.recent, a4 = a & ~3;
-  const int quads = (b - a4 + 3) >> 2;
+  // Candidates are tokens [a, b). Tokens are handled in quads - four neighbours share a page; this CTA has quads
+  // [q_first, q_last), keys[] holds theirs from q_first on.
+  const int a = p.sinks, b = len - p.recent;
+  const int all_quads = (len + 3) >> 2;
+  const int slice = (all_quads + cluster - 1) / cluster;
+  const int q_first = min(all_quads, rank * slice), q_last = min(all_quads, q_first + slice);
+  const int quads = q_last - q_first;
   const bool cached = quads * 4 <= p.cached_keys;
-  auto load_quad = [&](int i) {
-    const int t = a4 + 4 * i;
-    const int64_t block = table[t >> kKvBlockShift];
-    const float4 w = *reinterpret_cast<const float4*>(p.weights + (block * p.kv_heads + head) * kKvBlock + (t & (kKvBlock - 1)));
-    return make_uint4(OrderKey(w.x), OrderKey(w.y), OrderKey(w.z), OrderKey(w.w));
+  auto order = [](const float4& w) { return make_uint4(OrderKey(w.x), OrderKey(w.y), OrderKey(w.z), OrderKey(w.w)); };
+  auto weights_of = [&](int q, int block) {
+    return *reinterpret_cast<const float4*>(p.weights + (static_cast<int64_t>(block) * p.kv_heads + head) * kKvBlock + ((4 * q) & (kKvBlock - 1)));
   };
-  auto quad = [&](int i) { return cached ? reinterpret_cast<const uint4*>(keys)[i] : load_quad(i); };
-  auto clear_bins = [&]() {
-    for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
-  };
-  // every candidate key of this thread's quads
-  auto for_each = [&](auto&& quad_of, auto&& use) {
-#pragma unroll 4
-    for (int i = tid; i < quads; i += kSelectThreads) {
-      const uint4 k = quad_of(i);
-      const int t = a4 + 4 * i;
+  auto quad = [&](int q) { return cached ? reinterpret_cast<const uint4*>(keys)[q - q_first] : order(weights_of(q, table[q >> 2])); };
+  auto use_quad = [&](int q, const uint4& k, auto&& use) {
+    const int t = 4 * q;
+    if (t >= a && t + 3 < b) {
+      use(k.x), use(k.y), use(k.z), use(k.w);
+    } else {
       if (t >= a && t < b) use(k.x);
       if (t + 1 >= a && t + 1 < b) use(k.y);
       if (t + 2 >= a && t + 2 < b) use(k.z);
       if (t + 3 >= a && t + 3 < b) use(k.w);
     }
   };
+  auto for_each = [&](auto&& use) {
+#pragma unroll 4
+    for (int q = q_first + tid; q < q_last; q += kSelectThreads) use_quad(q, quad(q), use);
+  };
+  auto clear_bins = [&](int* bins) { bins[tid] = bins[tid + kSelectThreads] = 0; };
 
   // thr: tokens with a larger key stay, and the first `ties` of those whose key equals it
   uint32_t thr = 0xFFFFFFFFu;   // no weight has this key
   int ties = 0;
   int need = p.budget - p.sinks - p.recent;
   if (need > 0) {
-    clear_bins();
+    // The keys' range first, while they are fetched: bins that divide the RANGE spread over the candidates, where bins
+    // of leading bits would all be hit in the few octaves that attention weights lie in.
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    auto widen = [&](uint32_t k) {
+      lo = min(lo, k);
+      hi = max(hi, k);
+    };
+    clear_bins(sh.bins);
+    if (tid == 0) sh.listed = 0;
+#pragma unroll 1
+    for (int q0 = q_first + tid; q0 < q_last; q0 += kLoadAhead * kSelectThreads) {
+      int block[kLoadAhead];   // all table entries of a round in flight, then all weights
+      float4 w[kLoadAhead];
+#pragma unroll
+      for (int j = 0; j < kLoadAhead; ++j) block[j] = table[min(q0 + j * kSelectThreads, q_last - 1) >> 2];
+#pragma unroll
+      for (int j = 0; j < kLoadAhead; ++j) w[j] = weights_of(min(q0 + j * kSelectThreads, q_last - 1), block[j]);
+#pragma unroll
+      for (int j = 0; j < kLoadAhead; ++j) {
+        const int q = q0 + j * kSelectThreads;
+        if (q < q_last) {
+          const uint4 k = order(w[j]);
+          if (cached) reinterpret_cast<uint4*>(keys)[q - q_first] = k;
+          use_quad(q, k, widen);
+        }
+      }
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) {
+      warp_lo[warp] = lo;
+      warp_hi[warp] = hi;
+    }
     __syncthreads();
-    for_each([&](int i) {
-      const uint4 k = load_quad(i);
-      if (cached) reinterpret_cast<uint4*>(keys)[i] = k;
-      return k;
-    }, [&](uint32_t k) { atomicAdd(&bins[k >> 21], 1); });
-    uint32_t prefix = 0;
-    int shift = 21;   // of the digit in hand; the digits above it equal `prefix`
+    lo = __reduce_min_sync(0xffffffffu, warp_lo[lane]);
+    hi = __reduce_max_sync(0xffffffffu, warp_hi[lane]);
+    if (cluster > 1) {
+      if (tid == 0) {
+        sh.lo = lo;
+        sh.hi = hi;
+      }
+      ClusterBarrier();
+      lo = __reduce_min_sync(0xffffffffu, lane < cluster ? LoadPeer(&sh.lo, lane) : 0xFFFFFFFFu);
+      hi = __reduce_max_sync(0xffffffffu, lane < cluster ? LoadPeer(&sh.hi, lane) : 0u);
+    }
+    // Each round: the need-th largest key among those in [lo, hi] lies in one of up to 2048 bins of 2^shift keys. The
+    // counts of all CTAs are summed by each of them, which then go on alike.
+    uint32_t mine = 0;   // once the keys of one bin are listed: this thread's
+    int count = 0;       // of keys listed
 #pragma unroll 1
     while (true) {
-      __syncthreads();
-      // the bin that holds the need-th largest key: thread i sums bins 2047 - 2i and 2046 - 2i, from the top down
-      const int hi = bins[kBins - 1 - 2 * tid], lo = bins[kBins - 2 - 2 * tid];
-      int incl = hi + lo;
+      const int shift = max(0, 32 - __clz(hi - lo) - kBinBits);
+      int upper_bin, lower_bin;   // of thread i: bins 2047 - 2i and 2046 - 2i, from the top down
+      if (count == 0) {
+        for_each([&](uint32_t k) {
+          if (k >= lo && k <= hi) atomicAdd(&sh.bins[(k - lo) >> shift], 1);
+        });
+        upper_bin = lower_bin = 0;
+        if (cluster > 1) {
+          ClusterBarrier();
+          int2 pair[kMaxSelectCluster];   // all requests under way before the first is used
+#pragma unroll
+          for (int r = 0; r < kMaxSelectCluster; ++r) pair[r] = r < cluster ? LoadPeer2(&sh.bins[kBins - 2 - 2 * tid], r) : make_int2(0, 0);
+#pragma unroll
+          for (int r = 0; r < kMaxSelectCluster; ++r) {
+            upper_bin += pair[r].y;
+            lower_bin += pair[r].x;
+          }
+        } else {
+          __syncthreads();
+          upper_bin = sh.bins[kBins - 1 - 2 * tid];
+          lower_bin = sh.bins[kBins - 2 - 2 * tid];
+        }
+      } else {
+        clear_bins(local_bins);
+        __syncthreads();
+        if (tid < count && mine >= lo && mine <= hi) atomicAdd(&local_bins[(mine - lo) >> shift], 1);
+        __syncthreads();
+        upper_bin = local_bins[kBins - 1 - 2 * tid];
+        lower_bin = local_bins[kBins - 2 - 2 * tid];
+      }
+      int incl = upper_bin + lower_bin;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, off);
@@ -126,109 +235,165 @@ __global__ void __launch_bounds__(kSelectThreads) SelectKernel(const Params p) {
       }
       if (lane == 31) warp_sum[warp] = incl;
       __syncthreads();
-      int before = warp_sum[lane];   // lane w: the sum of warp w's bins
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, off);
-        if (lane >= off) before += v;
-      }
-      const int passed = __shfl_sync(0xffffffffu, before, warp > 0 ? warp - 1 : 0);
-      const int above = (warp > 0 ? passed : 0) + incl - hi - lo;
-      if (above < need && above + hi + lo >= need) {
-        const bool upper = above + hi >= need;
+      const int above = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0) + incl - upper_bin - lower_bin;
+      if (above < need && above + upper_bin + lower_bin >= need) {
+        const bool upper = above + upper_bin >= need;
         found_bin = kBins - 1 - 2 * tid - (upper ? 0 : 1);
-        found_above = above + (upper ? 0 : hi);
-        found_count = upper ? hi : lo;
+        found_above = above + (upper ? 0 : upper_bin);
+        found_count = upper ? upper_bin : lower_bin;
       }
       __syncthreads();
       need -= found_above;
-      prefix |= static_cast<uint32_t>(found_bin) << shift;
-      if (found_count == need) {   // all of this bin stay: whatever is below it does not
-        thr = prefix - 1;          // (never below 0: some candidate is left out)
+      lo += static_cast<uint32_t>(found_bin) << shift;
+      const int found = found_count;
+      if (found == need) {   // all of this bin stay: whatever is below it does not
+        thr = lo - 1;        // (never below 0: some candidate is left out)
         break;
       }
       if (shift == 0) {
-        thr = prefix;
+        thr = lo;
         ties = need;
         break;
       }
-      const int above_digit = shift;
-      shift = shift == 21 ? 10 : 0;
-      const uint32_t digit_mask = shift == 10 ? 0x7FFu : 0x3FFu;
-      __syncthreads();
-      clear_bins();
-      __syncthreads();
-      for_each(quad, [&](uint32_t k) {
-        if (((k ^ prefix) >> above_digit) == 0) atomicAdd(&bins[(k >> shift) & digit_mask], 1);
-      });
+      hi = min(hi, lo + ((1u << shift) - 1u));
+      if (count == 0 && found <= kListed) {
+        // Few enough to leave the crowd: every CTA lists its own, then copies the lists of all, in CTA order.
+        for_each([&](uint32_t k) {
+          if (k >= lo && k <= hi) sh.list[atomicAdd(&sh.listed, 1)] = k;
+        });
+        if (cluster > 1) ClusterBarrier(); else __syncthreads();
+        count = found;
+        int from = tid, r = 0;
+        if (cluster > 1) {
+          for (; r < cluster; ++r) {
+            const int theirs = static_cast<int>(LoadPeer(&sh.listed, r));
+            if (from < theirs) break;
+            from -= theirs;
+          }
+        }
+        if (tid < count) mine = cluster > 1 ? LoadPeer(&sh.list[from], r) : sh.list[from];
+      } else if (count == 0) {
+        if (cluster > 1) ClusterBarrier(); else __syncthreads();   // every peer has read these counts
+        clear_bins(sh.bins);
+        __syncthreads();
+        continue;
+      }
+      if (found <= kRanked) {   // rank the last few against one another
+        if (tid == 0) found_count = 0;
+        __syncthreads();
+        const bool in = tid < count && mine >= lo && mine <= hi;
+        if (in) crowd[atomicAdd(&found_count, 1)] = mine;
+        __syncthreads();
+        if (in) {
+          int larger = 0, equal = 0;
+          for (int i = 0; i < found; ++i) {
+            larger += crowd[i] > mine;
+            equal += crowd[i] == mine;
+          }
+          if (larger < need && larger + equal >= need) {   // every thread with this key says the same
+            found_key = mine;
+            found_above = larger;
+          }
+        }
+        __syncthreads();
+        thr = found_key;
+        ties = need - found_above;
+        break;
+      }
     }
   }
 
-  // ---- the kept positions in cache order: each warp a stretch of the sequence
+  // ---- the kept positions in cache order: each CTA its slice, each warp a stretch of it, four tokens per lane
   __syncthreads();
-  const int stretch = ((len + kSelectThreads - 1) / kSelectThreads) * 32;
-  const int t_begin = min(len, warp * stretch), t_end = min(len, t_begin + stretch);
-  auto key_at = [&](int t) -> uint32_t {
-    if (cached) return keys[t - a4];
-    const int64_t block = table[t >> kKvBlockShift];
-    return OrderKey(p.weights[(block * p.kv_heads + head) * kKvBlock + (t & (kKvBlock - 1))]);
-  };
-  // whether token t stays in any case, and whether it is one of the equals
-  auto judge = [&](int t, bool& sure, bool& equal) {
-    sure = equal = false;
-    if (t < t_end) {
-      if (t < a || t >= b) {
-        sure = true;
-      } else if (thr != 0xFFFFFFFFu) {
-        const uint32_t k = key_at(t);
-        sure = k > thr;
-        equal = k == thr && ties > 0;
+  const int stretch = ((quads + kSelectThreads - 1) / kSelectThreads) * 32;
+  const int q_begin = min(q_last, q_first + warp * stretch), q_end = min(q_last, q_begin + stretch);
+  // of the four tokens from 4q on, one bit each: those that stay in any case, and those whose key equals the threshold
+  auto judge = [&](int q, uint32_t& sure, uint32_t& equal) {
+    sure = equal = 0;
+    if (q >= q_end) return;
+    const int t = 4 * q;
+    const bool inside = t >= a && t + 3 < b;
+    uint4 k = make_uint4(0, 0, 0, 0);
+    if (t + 3 >= a && t < b) k = quad(q);
+    sure = (k.x > thr ? 1u : 0u) | (k.y > thr ? 2u : 0u) | (k.z > thr ? 4u : 0u) | (k.w > thr ? 8u : 0u);
+    equal = (k.x == thr ? 1u : 0u) | (k.y == thr ? 2u : 0u) | (k.z == thr ? 4u : 0u) | (k.w == thr ? 8u : 0u);
+    if (ties == 0) equal = 0;
+    if (!inside) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (t + e < a || t + e >= b) {   // not a candidate: stays if it is a token at all
+          sure |= 1u << e;
+          equal &= ~(1u << e);
+        }
+        if (t + e >= len) sure &= ~(1u << e);
       }
     }
   };
   int n_sure = 0, n_equal = 0;
 #pragma unroll 4
-  for (int t0 = t_begin; t0 < t_end; t0 += 32) {
-    bool sure, equal;
-    judge(t0 + lane, sure, equal);
-    n_sure += __popc(__ballot_sync(0xffffffffu, sure));
-    n_equal += __popc(__ballot_sync(0xffffffffu, equal));
+  for (int q0 = q_begin; q0 < q_end; q0 += 32) {
+    uint32_t sure, equal;
+    judge(q0 + lane, sure, equal);
+    n_sure += __popc(sure);
+    n_equal += __popc(equal);
   }
+  n_sure = __reduce_add_sync(0xffffffffu, n_sure);
+  n_equal = __reduce_add_sync(0xffffffffu, n_equal);
   if (lane == 0) {
     warp_sum[warp] = n_sure;
     warp_equal[warp] = n_equal;
   }
   __syncthreads();
-  int sure_before = lane < warp ? warp_sum[lane] : 0, equal_before = lane < warp ? warp_equal[lane] : 0;
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    sure_before += __shfl_xor_sync(0xffffffffu, sure_before, off);
-    equal_before += __shfl_xor_sync(0xffffffffu, equal_before, off);
+  int equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_equal[lane] : 0);
+  int sure_before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
+  if (cluster > 1) {
+    if (tid == kSelectThreads - 1) {
+      sh.sure = sure_before + warp_sum[warp];
+      sh.equal = equal_before + warp_equal[warp];
+    }
+    ClusterBarrier();
+    sure_before += __reduce_add_sync(0xffffffffu, lane < rank ? static_cast<int>(LoadPeer(&sh.sure, lane)) : 0);
+    equal_before += __reduce_add_sync(0xffffffffu, lane < rank ? static_cast<int>(LoadPeer(&sh.equal, lane)) : 0);
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (waited for at the end: a peer may still read)
   }
-  const uint32_t below = (1u << lane) - 1u;
   int at = sure_before + min(equal_before, ties);
 #pragma unroll 2
-  for (int t0 = t_begin; t0 < t_end; t0 += 32) {
-    bool sure, equal;
-    judge(t0 + lane, sure, equal);
-    const uint32_t equals = __ballot_sync(0xffffffffu, equal);
-    const bool keep = sure || (equal && equal_before + __popc(equals & below) < ties);
-    const uint32_t keeps = __ballot_sync(0xffffffffu, keep);
-    if (keep) kept[at + __popc(keeps & below)] = t0 + lane;
-    at += __popc(keeps);
-    equal_before += __popc(equals);
+  for (int q0 = q_begin; q0 < q_end; q0 += 32) {
+    uint32_t sure, equal;
+    judge(q0 + lane, sure, equal);
+    const uint32_t mine = __popc(sure) | __popc(equal) << 16;
+    uint32_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += v;
+    }
+    const uint32_t sum = __shfl_sync(0xffffffffu, incl, 31), excl = incl - mine;
+    const int stay = max(0, ties - equal_before);   // equals that still stay from here on
+    int left = stay - static_cast<int>(excl >> 16);
+    int j = at + static_cast<int>(excl & 0xFFFFu) + min(static_cast<int>(excl >> 16), stay);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool tie = (equal >> e) & 1u;
+      if (((sure >> e) & 1u) || (tie && left > 0)) kept[j++] = 4 * (q0 + lane) + e;
+      left -= tie;
+    }
+    at += static_cast<int>(sum & 0xFFFFu) + min(static_cast<int>(sum >> 16), stay);
+    equal_before += static_cast<int>(sum >> 16);
   }
+  if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 constexpr int kMoveThreads = 256;
 constexpr int kMoveWarps = kMoveThreads / 32;
-constexpr int kRowsInFlight = 16;
+constexpr int kRowsInFlight = 8;    // per warp, 512 bytes each; with four CTAs on an SM 128 KB are in flight
 constexpr int kCluster = 8;
 
 // kRowWords: 16-byte words of one token's K row and V row together when it is the same for every lane pattern (head_dim
 // 128: 32, one word per lane and row), 0 for any other width.
-template <bool kInPlace, int kRowWords>
-__global__ void __launch_bounds__(kMoveThreads) MoveKernel(const Params p, int parts) {
+// kLookup: rows a warp looks up at a time when not in place.
+template <bool kInPlace, int kRowWords, int kLookup>
+__global__ void __launch_bounds__(kMoveThreads, 4) MoveKernel(const Params p, int parts) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int seq = blockIdx.x / parts, part = blockIdx.x % parts, head = blockIdx.y;
@@ -247,7 +412,7 @@ __global__ void __launch_bounds__(kMoveThreads) MoveKernel(const Params p, int p
 
   // Rows a warp looks up and moves per round. In place all of them must be in registers before the first is written;
   // with one row per warp that holds for any width, since a word only ever moves to the same word of another row.
-  constexpr int kRows = !kInPlace ? 32 : kRowWords == 32 ? kRowsInFlight : 1;
+  constexpr int kRows = !kInPlace ? kLookup : kRowWords == 32 ? kRowsInFlight : 1;
   const int round = parts * kMoveWarps * kRows;
   for (int j0 = 0; j0 < n; j0 += round) {
     const int first = j0 + (part * kMoveWarps + warp) * kRows;
@@ -375,20 +540,31 @@ extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int
   p.budget = budget;
   p.sinks = sinks;
   p.recent = recent;
+  const int64_t items = static_cast<int64_t>(num_seqs) * num_kv_heads;
   p.cached_keys = static_cast<int>(tokens < kMaxCachedKeys ? tokens : kMaxCachedKeys);
   const int rc = EnsureReady(fn);
   if (rc != RL_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = LaunchDependent(SelectKernel, dim3(num_seqs, num_kv_heads), dim3(kSelectThreads),
-                                  static_cast<size_t>(p.cached_keys) * 4, 1, s, p);
+  // A cluster per item as far as the SMs go round and each CTA still has a few thousand tokens (as long as the table
+  // says the sequences may be).
+  int cluster = 1;
+  while (cluster < kMaxSelectCluster && 2 * cluster * items <= CurrentDeviceFacts().sm_count && tokens / (2 * cluster) >= kSelectThreads * 2)
+    cluster *= 2;
+  cudaError_t e = LaunchDependent(SelectKernel, dim3(static_cast<unsigned>(num_seqs) * cluster, num_kv_heads), dim3(kSelectThreads),
+                                  static_cast<size_t>(p.cached_keys) * 4, cluster, s, p, cluster);
   if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s: %s", fn, cudaGetErrorString(e));
   const bool in_place = dst_block_tables == block_tables;
-  const int64_t most = ((tokens < budget ? tokens : budget) + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
-  const int64_t items = static_cast<int64_t>(num_seqs) * num_kv_heads;
-  const int64_t fair = (16LL * CurrentDeviceFacts().sm_count + items - 1) / items;
+  // Out of place a warp looks 32 rows up and moves them eight at a time - or, while all rows then still fit the machine
+  // at once, only eight, so that no row waits for another.
+  const int64_t longest = tokens < budget ? tokens : budget;
+  const int sms = CurrentDeviceFacts().sm_count;
+  const bool few = items * longest <= 4LL * sms * kMoveWarps * kRowsInFlight;
+  const int rows = few ? kRowsInFlight : 32;
+  const int64_t most = (longest + kMoveWarps * rows - 1) / (kMoveWarps * rows);
+  const int64_t fair = (16LL * sms + items - 1) / items;
   const int parts = in_place ? kCluster : static_cast<int>(most < fair ? most : fair);
-  const bool plain = head_dim == 128;
-  auto kernel = in_place ? (plain ? MoveKernel<true, 32> : MoveKernel<true, 0>) : (plain ? MoveKernel<false, 32> : MoveKernel<false, 0>);
+  auto kernel = head_dim == 128 ? (in_place ? MoveKernel<true, 32, 0> : few ? MoveKernel<false, 32, kRowsInFlight> : MoveKernel<false, 32, 32>)
+                                : (in_place ? MoveKernel<true, 0, 0> : few ? MoveKernel<false, 0, kRowsInFlight> : MoveKernel<false, 0, 32>);
   e = LaunchDependent(kernel, dim3(static_cast<unsigned>(num_seqs) * parts, num_kv_heads), dim3(kMoveThreads), 0,
                       in_place ? kCluster : 1, s, p, parts);
   if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s (move): %s", fn, cudaGetErrorString(e));
