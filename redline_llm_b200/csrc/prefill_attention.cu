@@ -346,6 +346,7 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
   }
   auto key_pos = [&](int key) { return kWindow && key >= sink_pages * kKvBlock ? key + page_skip * kKvBlock : key; };
 
+  if (kWindow) asm volatile("griddepcontrol.wait;" ::: "memory");   // a dependent launch: set up under the previous kernel's tail
   // The loader's first table reads (lane l < 8 serves page l of a block) are under way before the CTA's barrier.
   auto table_entry = [&](int j) {
     const int entry = (jb0 + j) * kPagesPerBlock + lane;
@@ -1039,7 +1040,12 @@ int LaunchChunk(const char* fn, void* out, int64_t out_row_stride, const void* q
   p.scale_log2e = scale * 1.4426950408889634f;
   p.error_flag = st->error_flag;
   const dim3 grid(num_q_heads, static_cast<unsigned>(items));
-  PagedPrefillAttentionKernel<kWindow><<<grid, kThreads, kSmemBytes, stream>>>(p, q_map, page_map);
+  if (kWindow) {
+    const cudaError_t e = LaunchDependent(PagedPrefillAttentionKernel<kWindow>, grid, dim3(kThreads), kSmemBytes, 1, stream, p, q_map, page_map);
+    if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s: %s", fn, cudaGetErrorString(e));
+  } else {
+    PagedPrefillAttentionKernel<kWindow><<<grid, kThreads, kSmemBytes, stream>>>(p, q_map, page_map);
+  }
   rc = LaunchStatus(fn);
   if (rc != RL_OK || !any_split) return rc;
   // (a dependent launch whatever the process-wide switch says: the kernel begins with the wait for the stream's
