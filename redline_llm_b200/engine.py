@@ -153,6 +153,9 @@ class Request:
     cached: int = 0             # tokens in the cache (prompt + generated, except the pending one)
     finished: bool = False
     reason: str = ""
+    total_blocks: int = 0       # pages its longest cache would fill
+    need: int = 0               # pages it may hold at a time, reserved at admission
+    trimmed: int = 0            # pages from here on have not been looked at by trim()
 
     @property
     def seq_len(self) -> int:   # tokens the next decode step attends to, including the new one
@@ -160,10 +163,13 @@ class Request:
 
 
 class Scheduler:
-    """FCFS admission, prefill-before-decode, bucketed decode batches."""
+    """FCFS admission, prefill-before-decode, bucketed decode batches. With an attention window a request holds - and
+    reserves - only the pages some later query can see: the sinks' and the window's; pages that fall behind go back
+    to the allocator (trim)."""
 
     def __init__(self, allocator: BlockAllocator, max_batch: int, max_seq_len: int, prefill_chunk: int,
-                 eos_token_id=151645):
+                 eos_token_id=151645, window: int = 0, sinks: int = 0):
+        self.window, self.sinks = window, sinks      # window 0: every query sees the whole cache
         self.alloc, self.max_batch, self.max_seq_len, self.chunk = allocator, max_batch, max_seq_len, prefill_chunk
         # one id or the whole stop set; compared as a set (src/core/scheduler.cpp: IsEosToken)
         self.eos = frozenset([eos_token_id] if isinstance(eos_token_id, int) else eos_token_id)
@@ -177,7 +183,8 @@ class Scheduler:
     def _admit(self) -> None:
         while self.waiting and len(self.running) < self.max_batch:
             r = self.waiting[0]
-            need = blocks_for_tokens(len(r.prompt) + r.max_new_tokens)
+            total = blocks_for_tokens(len(r.prompt) + r.max_new_tokens)
+            need = min(total, self.held_blocks())
             if not self.alloc.can_reserve(need):
                 if not self.running:  # can never fit: abort instead of stalling forever
                     self.waiting.popleft()
@@ -186,8 +193,34 @@ class Scheduler:
                     self.running.append(r)
                 return
             self.alloc.reserve(need)
-            r.reserved_left = need
+            r.reserved_left = r.need = need
+            r.total_blocks = total
             self.running.append(self.waiting.popleft())
+
+    def held_blocks(self) -> int:
+        """The most pages a request can hold at a time: without a window any number; with one, the sinks' pages and
+        those of the window plus what is written ahead of it - a prompt chunk, or the two decode steps in flight."""
+        if not self.window:
+            return 1 << 30
+        return blocks_for_tokens(self.sinks) + blocks_for_tokens(self.window + max(self.chunk, 2)) + 1
+
+    def trim(self, r: Request, next_position: int) -> None:
+        """Gives back the pages of `r` that no query at `next_position` or later sees, and keeps as many reserved as
+        the request may still grow into. Their table entries become the padding block: the window kernels read neither."""
+        if not self.window:
+            return
+        first = max(r.trimmed, blocks_for_tokens(self.sinks))
+        last = max(0, next_position - self.window + 1) // KV_BLOCK
+        for k in range(first, min(last, len(r.blocks))):
+            if r.blocks[k] != DUMMY_BLOCK:
+                self.alloc.free_block(r.blocks[k])
+                r.blocks[k] = DUMMY_BLOCK
+        r.trimmed = max(r.trimmed, last)
+        live = sum(1 for b in r.blocks if b != DUMMY_BLOCK)
+        more = min(r.need - live, r.total_blocks - len(r.blocks)) - r.reserved_left
+        if more > 0:
+            self.alloc.reserve(more)
+            r.reserved_left += more
 
     def _grow(self, r: Request, tokens: int) -> None:
         while len(r.blocks) < blocks_for_tokens(tokens):
@@ -231,7 +264,8 @@ class Scheduler:
 
     def release(self, r: Request) -> None:
         for b in r.blocks:
-            self.alloc.free_block(b)
+            if b != DUMMY_BLOCK:
+                self.alloc.free_block(b)
         r.blocks = []
         self.alloc.unreserve(r.reserved_left)
         r.reserved_left = 0
@@ -316,6 +350,9 @@ class ModelExecutor:
         self.attention_events = None  # set by profile runs
         self.prefill_logits = None
         self.prefill_attention = "fused"   # or "composite": gather -> library GEMM -> softmax -> library GEMM
+        # Sliding window and sinks of every layer's attention (0: the whole cache); set before warm_and_capture.
+        self.attention_window, self.attention_sinks = 0, 0
+        self.window_ws = self.prefill_ws = None   # workspaces of the window kernels: this executor launches on one stream
         self.fuse_rope_scatter = True  # one launch for RoPE + scatter; False = the reference's two launches
         # Linear layers of the decode step: "tcgen05" = this library's weight-streaming kernel (with the
         # SiLU-mul fused into the gate/up product), "library" = torch.matmul (cuBLAS), as the reference.
@@ -363,9 +400,15 @@ class ModelExecutor:
             if self.attention_events is not None:
                 e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
                 e0.record()
-            K.launch_paged_attention_decode(attn, cfg.q_width, qkv, cfg.qkv_width, self.pool[li], self.tables,
-                                            self.seq_lens, rows, self.mbps, cfg.q_heads, cfg.kv_heads,
-                                            cfg.head_dim, self.scale)
+            if self.attention_window:
+                K.launch_paged_window_attention_decode(attn, cfg.q_width, qkv, cfg.qkv_width, self.pool[li], self.tables,
+                                                       self.seq_lens, rows, self.mbps, cfg.q_heads, cfg.kv_heads,
+                                                       cfg.head_dim, self.scale, self.attention_window,
+                                                       self.attention_sinks, self.window_ws)
+            else:
+                K.launch_paged_attention_decode(attn, cfg.q_width, qkv, cfg.qkv_width, self.pool[li], self.tables,
+                                                self.seq_lens, rows, self.mbps, cfg.q_heads, cfg.kv_heads,
+                                                cfg.head_dim, self.scale)
             if self.attention_events is not None:
                 e1.record()
                 self.attention_events.append((e0, e1))
@@ -397,6 +440,9 @@ class ModelExecutor:
     def warm_and_capture(self, buckets: Sequence[int]) -> None:
         """Eager warm-up of every bucket (first launches happen outside capture), then one graph each."""
         torch = self.torch
+        if self.attention_window:
+            self.window_ws = self.K.window_attention_workspace(BUCKETS[-1], self.mbps, self.cfg.q_heads,
+                                                               self.cfg.kv_heads, device=self.device)
         self.seq_lens.fill_(1)
         for b in buckets:
             self.enqueue_decode(b)
@@ -536,6 +582,11 @@ class ModelExecutor:
         fused = (self.prefill_attention == "fused" and cfg.head_dim == 128
                  and hasattr(K, "launch_paged_prefill_attention"))
         group = cfg.q_heads // cfg.kv_heads
+        window, sinks = self.attention_window, self.attention_sinks
+        if window:
+            need = K.window_prefill_workspace_bytes(start, n, cfg.q_heads, window, sinks)
+            if self.prefill_ws is None or self.prefill_ws.nbytes < need:
+                self.prefill_ws = K.window_prefill_workspace(start, n, cfg.q_heads, window, sinks, device=dev)
         if fused:
             attn = torch.empty(n, cfg.q_width, dtype=torch.float16, device=dev)
         else:
@@ -553,7 +604,11 @@ class ModelExecutor:
             K.launch_kv_scatter(self.pool[li], qkv, qkv, cfg.qkv_width, cfg.qkv_width, row, 0, pos, n,
                                 cfg.kv_heads, cfg.head_dim, k_offset=cfg.q_width,
                                 v_offset=cfg.q_width + cfg.kv_width)
-            if fused:
+            if window:
+                K.launch_paged_window_prefill_attention(attn, cfg.q_width, qkv, cfg.qkv_width, self.pool[li], row, self.mbps,
+                                                        start, n, cfg.q_heads, cfg.kv_heads, cfg.head_dim, self.scale,
+                                                        window, sinks, self.prefill_ws)
+            elif fused:
                 K.launch_paged_prefill_attention(attn, cfg.q_width, qkv, cfg.qkv_width, self.pool[li], row, self.mbps,
                                                  start, n, cfg.q_heads, cfg.kv_heads, cfg.head_dim, self.scale)
             else:
@@ -591,12 +646,17 @@ class Engine:
                  device: int = 0, seed: int = 0x5EED, weights: Optional[ModelWeights] = None,
                  graph_buckets: Optional[Sequence[int]] = None, prologue_overlap: bool = True,
                  decode_linear: str = "tcgen05", vocab_projection: Optional[str] = None,
-                 device_feedback: bool = True, prefill_attention: str = "fused"):
+                 device_feedback: bool = True, prefill_attention: str = "fused", attention_window: int = 0,
+                 attention_sinks: int = 0):
         import torch
         if admission_policy != "reserve_full":
             raise ValueError("only the reserve_full admission policy is provided")
         if not 1 <= max_batch <= BUCKETS[-1]:
             raise ValueError(f"max_batch must be in [1, {BUCKETS[-1]}]")
+        if attention_window < 0 or attention_sinks < 0 or (attention_sinks and not attention_window):
+            raise ValueError("attention_window and attention_sinks must be >= 0, and sinks need a window")
+        if attention_window and prefill_attention != "fused":
+            raise ValueError("an attention window needs prefill_attention='fused'")
         if model_dir is not None:
             raise ValueError("checkpoint loading is outside this library: pass weights= or use random init")
         if not torch.cuda.is_available():
@@ -607,7 +667,8 @@ class Engine:
         num_blocks = max(2, int(kv_pool_gb * (1 << 30)) // self.cfg.block_bytes())
         self.allocator = BlockAllocator(num_blocks)
         self.scheduler = Scheduler(self.allocator, max_batch, max_seq_len, prefill_chunk,
-                                   (self.cfg.eos_token_id,) + tuple(self.cfg.extra_eos_token_ids))
+                                   (self.cfg.eos_token_id,) + tuple(self.cfg.extra_eos_token_ids),
+                                   attention_window, attention_sinks)
         from . import kernels as K
         # attention's table walk may overlap the RoPE+scatter kernel before it: seq_lens and the block
         # tables are uploaded at the start of a step, never written by that kernel
@@ -617,6 +678,7 @@ class Engine:
             raise ValueError("decode_linear must be 'tcgen05' or 'library'")
         self.exec = ModelExecutor(self.cfg, self.weights, num_blocks, max_seq_len, self.device, enable_cuda_graphs)
         self.exec.decode_linear = decode_linear
+        self.exec.attention_window, self.exec.attention_sinks = int(attention_window), int(attention_sinks)
         self.exec.vocab_projection = vocab_projection or decode_linear
         if prefill_attention not in ("fused", "composite"):
             raise ValueError("prefill_attention must be 'fused' or 'composite'")
@@ -681,6 +743,7 @@ class Engine:
             _, r, start, end = plan
             tok = self.exec.prefill_chunk(r, start, end)
             self._stats["prefill_tokens"] += end - start
+            self.scheduler.trim(r, end)
             if tok is None:
                 self._queue.append(("done", []))
                 return
@@ -793,6 +856,8 @@ class Engine:
             r.cached += 1
             self._stats["decode_tokens"] += 1
             out.append(self.scheduler.complete(r, t))
+            if not r.finished:
+                self.scheduler.trim(r, r.cached)
         # what the next step feeds back: the APPENDED tokens (the scripted ones under teacher forcing); any
         # finished request changes the batch, which fill_mirrors notices by itself
         self.exec._last_tokens = np.fromiter((r.output[-1] for r in batch), dtype=np.int32, count=len(batch))
@@ -825,7 +890,7 @@ class Engine:
         r = Request(self._next_id, [seed % self.cfg.vocab], max_new_tokens, ignore_eos=True)
         self._next_id += 1
         self.allocator.reserve(need)
-        r.reserved_left = need
+        r.reserved_left = r.need = r.total_blocks = need
         self.scheduler._grow(r, context_len + 1)
         nb = blocks_for_tokens(context_len)
         if nb:
