@@ -48,6 +48,10 @@ static_assert(kWarps == kMaxGroup && kHeadDim == 4 * 32, "a fold gives each warp
 constexpr int kInlineOthers = 3;     // items over at most this many other CTAs are merged from registers
 constexpr int kMergeBatch = 16;      // longer ones: records in flight per thread
 constexpr int kMinPagesPerCta = kWarps;
+constexpr int kMinChunk = 2 * kWarps;      // an item is not cut finer than this ...
+constexpr int kWholeItem = 3 * kWarps;     // ... and not at all up to this: a ring holds three pages per warp, and handing over
+                                           // costs 1 us (300 tokens: 6.65 us whole, 7.73 in two; 8000 tokens: 11.5 us in
+                                           // chunks of 16 pages, 14.8 in chunks of 8, 11.6 in chunks of 32)
 constexpr int kSegmentPages = 12;    // what a second item costs a CTA (fold and hand-over, 2-3 us), in pages
 constexpr int kMaxCtas = 256;
 constexpr int kNewestPageBit = 1 << 30;
@@ -212,13 +216,13 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   if (items < static_cast<int>(gridDim.x)) {
     const int spare = static_cast<int>(gridDim.x) - items;
     const long long fit = (total + spare - 1) / spare;   // sum of ceil(pages / fit) <= total / fit + items <= the grid
-    longest = static_cast<int>(max(min(fit, static_cast<long long>(most_pages)), static_cast<long long>(kMinPagesPerCta)));
-    chunked = longest <= total / static_cast<int>(gridDim.x) + kSegmentPages;
+    longest = static_cast<int>(max(min(fit, static_cast<long long>(most_pages)), static_cast<long long>(kMinChunk)));
+    chunked = longest <= max(total / static_cast<int>(gridDim.x), static_cast<long long>(kMinChunk)) + kSegmentPages;
   }
   long long share_begin, share_end;
   int ctas, chunk_first = 0, chunk_last = 0;   // (chunked) the CTAs of this CTA's item
   if (chunked) {
-    const int chunks = my_pages > 0 ? (my_pages + longest - 1) / longest : 0;
+    const int chunks = my_pages > kWholeItem ? (my_pages + longest - 1) / longest : my_pages > 0 ? 1 : 0;
     const int incl = scan_sequences(chunks, warp_chunks);
     if (tid < kMaxSeqsPerLaunch) chunk_prefix[tid + 1] = incl;
     __syncthreads();

@@ -105,10 +105,20 @@ def _ptr(t, offset_elems: int = 0) -> int:
     return t.data_ptr() + 2 * offset_elems if t is not None else 0
 
 
+_current_stream = None   # the current device's current stream as an integer
+
+
 def _stream(stream) -> int:
+    global _current_stream
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        if _current_stream is None:
+            import torch
+            # Asking for the handle alone takes 0.3 us; the stream object around it takes 3.3 us, a third of the
+            # host's time for a small launch.
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+            _current_stream = ((lambda: raw(torch.cuda.current_device())) if raw is not None
+                               else (lambda: torch.cuda.current_stream().cuda_stream))
+        return _current_stream()
     return getattr(stream, "cuda_stream", stream)
 
 
