@@ -112,26 +112,31 @@ __device__ __forceinline__ int LoadAcquire(const int* p) {
   return v;
 }
 
-// Flattened pages: sequence-major, then KV head, then the item's page list.
-__device__ __forceinline__ long long ShareBegin(long long c, long long total, int ctas) { return c * total / ctas; }
-__device__ __forceinline__ int ShareOf(long long t, long long total, int ctas) {
-  return static_cast<int>(((t + 1) * ctas - 1) / total);
+// Flattened pages: sequence-major, then KV head, then the item's page list; the launcher keeps their number inside 31 bits.
+// n pages in `parts` equal parts: the first n % parts have one more.
+__device__ __forceinline__ int PartBegin(int part, int n, int parts) {
+  const int each = n / parts;
+  return part * each + min(part, n - each * parts);
+}
+__device__ __forceinline__ int PartOf(int page, int n, int parts) {   // the inverse; n >= parts
+  const int each = n / parts, longer = n - each * parts, there = longer * (each + 1);
+  return page < there ? page / (each + 1) : longer + (page - there) / each;
 }
 struct Cursor {
   int seq, head, entry, entries;   // entry of the item's page list, which has `entries`
 };
-__device__ __forceinline__ Cursor Locate(long long t, const int* prefix, int num_seqs, int heads) {
+__device__ __forceinline__ Cursor Locate(int t, const int* prefix, int num_seqs, int heads) {
   int lo = 0, hi = num_seqs - 1;
   while (lo < hi) {   // the first sequence whose pages end behind t
     const int mid = (lo + hi) >> 1;
-    if (static_cast<long long>(heads) * prefix[mid + 1] <= t) lo = mid + 1; else hi = mid;
+    if (heads * prefix[mid + 1] <= t) lo = mid + 1; else hi = mid;
   }
   Cursor c;
   c.seq = lo;
   c.entries = prefix[lo + 1] - prefix[lo];
-  const long long rem = t - static_cast<long long>(heads) * prefix[lo];
-  c.head = static_cast<int>(rem / c.entries);
-  c.entry = static_cast<int>(rem - static_cast<long long>(c.head) * c.entries);
+  const int rem = t - heads * prefix[lo];
+  c.head = rem / c.entries;
+  c.entry = rem - c.head * c.entries;
   return c;
 }
 
@@ -195,7 +200,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
     if (tid == 0) prefix[0] = chunk_prefix[0] = 0;
     __syncthreads();
   }
-  const long long total = static_cast<long long>(heads) * prefix[p.num_seqs];
+  const int total = heads * prefix[p.num_seqs];
   if (total == 0) {
     asm volatile("griddepcontrol.wait;" ::: "memory");   // this grid never completes ahead of the one before it
     return;
@@ -215,11 +220,11 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   bool chunked = false;
   if (items < static_cast<int>(gridDim.x)) {
     const int spare = static_cast<int>(gridDim.x) - items;
-    const long long fit = (total + spare - 1) / spare;   // sum of ceil(pages / fit) <= total / fit + items <= the grid
-    longest = static_cast<int>(max(min(fit, static_cast<long long>(most_pages)), static_cast<long long>(kMinChunk)));
-    chunked = longest <= max(total / static_cast<int>(gridDim.x), static_cast<long long>(kMinChunk)) + kSegmentPages;
+    const int fit = (total - 1) / spare + 1;   // sum of ceil(pages / fit) <= total / fit + items <= the grid
+    longest = max(min(fit, most_pages), kMinChunk);
+    chunked = longest <= max(total / static_cast<int>(gridDim.x), kMinChunk) + kSegmentPages;
   }
-  long long share_begin, share_end;
+  int share_begin, share_end;
   int ctas, chunk_first = 0, chunk_last = 0;   // (chunked) the CTAs of this CTA's item
   if (chunked) {
     const int chunks = my_pages > kWholeItem ? (my_pages + longest - 1) / longest : my_pages > 0 ? 1 : 0;
@@ -228,16 +233,16 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
     __syncthreads();
     ctas = heads * chunk_prefix[p.num_seqs];   // <= total / longest + items <= gridDim.x
     const Cursor c = Locate(cta < ctas ? cta : 0, chunk_prefix, p.num_seqs, heads);   // entry = chunk, entries = chunks
-    const long long pages = prefix[c.seq + 1] - prefix[c.seq];
-    const long long item = static_cast<long long>(heads) * prefix[c.seq] + c.head * pages;
-    share_begin = item + c.entry * pages / c.entries;
-    share_end = item + (c.entry + 1) * pages / c.entries;
+    const int pages = prefix[c.seq + 1] - prefix[c.seq];
+    const int item = heads * prefix[c.seq] + c.head * pages;
+    share_begin = item + PartBegin(c.entry, pages, c.entries);
+    share_end = item + PartBegin(c.entry + 1, pages, c.entries);
     chunk_first = cta - c.entry;
     chunk_last = chunk_first + c.entries - 1;
   } else {
-    ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(1LL, total / kMinPagesPerCta)));
-    share_begin = ShareBegin(cta, total, ctas);
-    share_end = ShareBegin(cta + 1, total, ctas);
+    ctas = min(static_cast<int>(gridDim.x), max(1, total / kMinPagesPerCta));
+    share_begin = PartBegin(cta, total, ctas);
+    share_end = PartBegin(cta + 1, total, ctas);
   }
   if (cta >= ctas) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -245,7 +250,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   }
 
   // ---- this warp's pages: share-relative indices warp, warp + 8, ...
-  const int share_len = static_cast<int>(share_end - share_begin);
+  const int share_len = share_end - share_begin;
   const int n_mine = share_len > warp ? (share_len - warp + kWarps - 1) / kWarps : 0;
   const uint32_t my_ring = SmemAddr(smem) + warp * (kStages * kStageBytes);
   const uint32_t my_bars = SmemAddr(smem + kBarOff) + warp * (kStages * 8);
@@ -258,7 +263,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   auto fetch_tiles = [&](int batch) -> int {
     const int k = 32 * batch + lane;
     if (k >= n_mine) return 0;
-    const Cursor c = Locate(share_begin + warp + static_cast<long long>(kWarps) * k, prefix, p.num_seqs, heads);
+    const Cursor c = Locate(share_begin + warp + kWarps * k, prefix, p.num_seqs, heads);
     const int page = c.entry >= p.sink_pages ? c.entry + skip[c.seq] : c.entry;
     const int block = __ldg(p.tables + static_cast<int64_t>(c.seq) * p.max_blocks + page);
     return (block * 2 * heads + c.head) | (c.entry == c.entries - 1 ? kNewestPageBit : 0);
@@ -312,17 +317,17 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   constexpr uint32_t kHiDims = 2048;
 
   // ---- one (sequence, KV head) segment of the share after the other
-  long long seg_begin = share_begin;
+  int seg_begin = share_begin;
 #pragma unroll 1
   while (seg_begin < share_end) {
     const Cursor sc = Locate(seg_begin, prefix, p.num_seqs, heads);
-    const long long item_begin = seg_begin - sc.entry, item_end = item_begin + sc.entries;
-    const long long seg_end = item_end < share_end ? item_end : share_end;
+    const int item_begin = seg_begin - sc.entry, item_end = item_begin + sc.entries;
+    const int seg_end = item_end < share_end ? item_end : share_end;
     const int len = min(p.seq_lens[sc.seq], p.max_blocks * kKvBlock);
     const int w0 = max(0, len - p.window);   // first token of the window
     const int gap = skip[sc.seq];
-    const int seg_end_rel = static_cast<int>(seg_end - share_begin);
-    const int entry0 = sc.entry - static_cast<int>(seg_begin - share_begin);   // entry of the share's page `rel` is rel + entry0
+    const int seg_end_rel = seg_end - share_begin;
+    const int entry0 = sc.entry - (seg_begin - share_begin);   // entry of the share's page `rel` is rel + entry0
     uint32_t qb[8][2];   // B operand of S^T: query g of the group in column g, zeros past the group
     {
       const half* qrow = p.q + static_cast<int64_t>(sc.seq) * p.q_stride +
@@ -339,8 +344,8 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
       c_first = chunk_first;
       c_last = chunk_last;
     } else if (!whole) {
-      if (item_begin < share_begin) c_first = ShareOf(item_begin, total, ctas);
-      if (item_end > share_end) c_last = ShareOf(item_end - 1, total, ctas);
+      if (item_begin < share_begin) c_first = PartOf(item_begin, total, ctas);
+      if (item_end > share_end) c_last = PartOf(item_end - 1, total, ctas);
     }
     const int others = c_last - c_first;
     const bool may_read_inline = !whole && others <= kInlineOthers;
@@ -804,8 +809,9 @@ int Launch(const Call& c) {
   // No more CTAs than shares of kMinPagesPerCta pages can exist: a row's list is at most this long.
   const int64_t list = p.sink_pages + ((p.window + kKvBlock - 2) >> kKvBlockShift) + 1;
   const int64_t pages = list < c.max_blocks ? list : c.max_blocks;
-  if (pages * kMaxSeqsPerLaunch > INT32_MAX && pages * c.num_seqs > INT32_MAX)
-    return Fail(RL_E_TOO_LARGE, "%s: more than 2^31 pages in one call", c.fn);
+  const int64_t rows = c.num_seqs < kMaxSeqsPerLaunch ? c.num_seqs : kMaxSeqsPerLaunch;
+  if (pages * rows * c.kv_heads > INT32_MAX - 65536)
+    return Fail(RL_E_TOO_LARGE, "%s: more than 2^31 pages (times KV heads) in one launch", c.fn);
   const int sms = CurrentDeviceFacts().sm_count < kMaxCtas ? CurrentDeviceFacts().sm_count : kMaxCtas;
   const int64_t row = static_cast<int64_t>(c.q_heads) * c.max_blocks * kKvBlock;
   for (int first = 0; first < c.num_seqs; first += kMaxSeqsPerLaunch) {
