@@ -387,13 +387,14 @@ __global__ void __launch_bounds__(kSelectThreads, 1) SelectKernel(const Params p
 constexpr int kMoveThreads = 256;
 constexpr int kMoveWarps = kMoveThreads / 32;
 constexpr int kRowsInFlight = 8;    // per warp, 512 bytes each; with four CTAs on an SM 128 KB are in flight
+constexpr int kWideWarps = 16, kWideRows = 16;   // in place with few items: a CTA has its SM to itself
 constexpr int kCluster = 8;
 
 // kRowWords: 16-byte words of one token's K row and V row together when it is the same for every lane pattern (head_dim
 // 128: 32, one word per lane and row), 0 for any other width.
-// kLookup: rows a warp looks up at a time when not in place.
-template <bool kInPlace, int kRowWords, int kLookup>
-__global__ void __launch_bounds__(kMoveThreads, 4) MoveKernel(const Params p, int parts) {
+// kLookup: rows a warp looks up at a time; in place (the K = 128 form) also the rows it has in registers at a time.
+template <bool kInPlace, int kRowWords, int kLookup, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps > kMoveWarps ? 1 : 4) MoveKernel(const Params p, int parts) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int seq = blockIdx.x / parts, part = blockIdx.x % parts, head = blockIdx.y;
@@ -412,10 +413,11 @@ __global__ void __launch_bounds__(kMoveThreads, 4) MoveKernel(const Params p, in
 
   // Rows a warp looks up and moves per round. In place all of them must be in registers before the first is written;
   // with one row per warp that holds for any width, since a word only ever moves to the same word of another row.
-  constexpr int kRows = !kInPlace ? kLookup : kRowWords == 32 ? kRowsInFlight : 1;
-  const int round = parts * kMoveWarps * kRows;
+  constexpr int kRows = !kInPlace || kRowWords == 32 ? kLookup : 1;
+  constexpr int kFlight = kInPlace ? kRows : kRowsInFlight;
+  const int round = parts * kWarps * kRows;
   for (int j0 = 0; j0 < n; j0 += round) {
-    const int first = j0 + (part * kMoveWarps + warp) * kRows;
+    const int first = j0 + (part * kWarps + warp) * kRows;
     const int rows = max(0, min(kRows, n - first));
     int64_t from = 0, to = 0, weight_to = 0;
     float weight = 0.0f;
@@ -433,10 +435,10 @@ __global__ void __launch_bounds__(kMoveThreads, 4) MoveKernel(const Params p, in
     if (kRowWords == 32) {
       const int64_t mine = lane < 16 ? lane : v_words + lane - 16;   // this lane's word of a row: K, then V
 #pragma unroll
-      for (int r0 = 0; r0 < kRows; r0 += kRowsInFlight) {
-        uint4 v[kRowsInFlight];
+      for (int r0 = 0; r0 < kRows; r0 += kFlight) {
+        uint4 v[kFlight];
 #pragma unroll
-        for (int r = 0; r < kRowsInFlight; ++r) {
+        for (int r = 0; r < kFlight; ++r) {
           const int64_t src = __shfl_sync(0xffffffffu, from, r0 + r);
           if ((moving >> (r0 + r)) & 1) v[r] = pool[src + mine];
         }
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) MoveKernel(const Params p, in
           asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         }
 #pragma unroll
-        for (int r = 0; r < kRowsInFlight; ++r) {
+        for (int r = 0; r < kFlight; ++r) {
           const int64_t d = __shfl_sync(0xffffffffu, to, r0 + r);
           if ((moving >> (r0 + r)) & 1) pool[d + mine] = v[r];
         }
@@ -563,9 +565,16 @@ extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int
   const int64_t most = (longest + kMoveWarps * rows - 1) / (kMoveWarps * rows);
   const int64_t fair = (16LL * sms + items - 1) / items;
   const int parts = in_place ? kCluster : static_cast<int>(most < fair ? most : fair);
-  auto kernel = head_dim == 128 ? (in_place ? MoveKernel<true, 32, 0> : few ? MoveKernel<false, 32, kRowsInFlight> : MoveKernel<false, 32, 32>)
-                                : (in_place ? MoveKernel<true, 0, 0> : few ? MoveKernel<false, 0, kRowsInFlight> : MoveKernel<false, 0, 32>);
-  e = LaunchDependent(kernel, dim3(static_cast<unsigned>(num_seqs) * parts, num_kv_heads), dim3(kMoveThreads), 0,
+  // In place a cluster's round is all that its registers hold. While every item's cluster has SMs to itself, rounds of 2048
+  // rows, 256 of them in the registers of each CTA; where the items fill the machine several times over, small CTAs, four to
+  // an SM, whose rounds overlap (one sequence of 32768 tokens to 8192: 36.0 us wide, 46.9 small; 64 sequences to 2048 stay small: 52.6).
+  const bool wide = in_place && items * kCluster <= sms;
+  auto kernel = head_dim == 128
+                    ? (wide ? MoveKernel<true, 32, kWideRows, kWideWarps> : in_place ? MoveKernel<true, 32, kRowsInFlight, kMoveWarps>
+                       : few ? MoveKernel<false, 32, kRowsInFlight, kMoveWarps> : MoveKernel<false, 32, 32, kMoveWarps>)
+                    : (wide ? MoveKernel<true, 0, 0, kWideWarps> : in_place ? MoveKernel<true, 0, 0, kMoveWarps>
+                       : few ? MoveKernel<false, 0, kRowsInFlight, kMoveWarps> : MoveKernel<false, 0, 32, kMoveWarps>);
+  e = LaunchDependent(kernel, dim3(static_cast<unsigned>(num_seqs) * parts, num_kv_heads), dim3(wide ? kWideWarps * 32 : kMoveThreads), 0,
                       in_place ? kCluster : 1, s, p, parts);
   if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s (move): %s", fn, cudaGetErrorString(e));
   return LaunchStatus(fn);
