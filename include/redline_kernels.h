@@ -49,8 +49,8 @@ const char* rl_last_error(void);
 
 /*
  * Optional warm-up for `device` (-1 = current): caches the SM count, opts the
- * attention kernel in to its dynamic shared memory and allocates the attention
- * workspace. The launchers do the same lazily on their first call; an engine
+ * attention, linear and eviction kernels in to their dynamic shared memory and allocates the attention
+ * workspace and error flags. The launchers do the same lazily on their first call; an engine
  * calls this (or performs one eager launch of each kernel, as the reference's
  * bucket warm-up does, src/core/model_executor.cpp:504-521) before capture.
  * No counterpart in the reference (its kernels keep no per-device state but
@@ -343,9 +343,9 @@ int rl_decode_linear_set_max_splits(int max_splits);
  * `window` tokens up to and including p:  V(p) = { t <= p : t < sinks or t > p - window }  (window >= 1, sinks >= 0;
  * a window that covers the sequence is plain causal attention). Shared by the three attention launchers below:
  * head_dim 128, 1 to 8 KV heads with 1 to 8 query heads each, scale positive and finite, FP32 scores, statistics and
- * accumulation, masking by SELECT (what invisible slots hold - NaN included - reaches no result), one FP16 rounding of
- * the output. Pages that hold no visible token are not read, and neither are their block-table entries: a caller may
- * have given them to other sequences. None of the four has a counterpart in the reference (full causal attention over
+ * accumulation, masking by SELECT (what a slot that no row of the call sees holds - NaN included - reaches no result), one
+ * FP16 rounding of the output; out overlaps neither q nor the pool. Pages that hold no visible token are not read, and
+ * neither are their block-table entries: a caller may have given them to other sequences. None of the four has a counterpart in the reference (full causal attention over
  * a cache that only grows, src/kernels/kernels.cuh:125-187 there).
  *
  * Workspaces are the caller's: device memory, 16-byte aligned, of at least the size that the matching query names,
@@ -402,7 +402,9 @@ int rl_window_prefill_workspace_bytes(int32_t chunk_start, int32_t chunk_len, in
 /*
  * rl_launch_paged_prefill_attention with a sliding window and sinks: row i of the chunk, at position chunk_start + i,
  * sees V(chunk_start + i). Only block-table entries of pages some row of the chunk sees are read. Same alignment rules
- * (q, out and the pool slice 16-byte aligned, row strides multiples of 8); num_q_heads / num_kv_heads at most 8.
+ * (q, out and the pool slice 16-byte aligned, row strides multiples of 8); num_q_heads / num_kv_heads at most 8. As in
+ * that launcher a token's V row meets every row of a 128-row query tile, with weight zero where the row does not see it:
+ * a V that is not finite and that SOME row of the tile sees makes NaN of the tile's other rows too.
  * workspace may be NULL (or smaller than the query names): then no (query tile, head) pair is cut into runs, which
  * only costs time. Its bounded waits report through rl_prefill_attention_health.
  */
@@ -422,7 +424,8 @@ int rl_launch_paged_window_prefill_attention(void* out, int64_t out_row_stride, 
  * kept[s][h][j] (int32 [num_seqs, num_kv_heads, budget]) is the slot that kept token j of head h had, -1 for j >= L'.
  *   dst_block_tables == block_tables: in place (pages behind the first ceil(L' / 16) are then free to reuse).
  *   any other dst_block_tables: its pages must be apart from every page of the source tables; the source stays as it is.
- * In either case a page belongs to one sequence of the call. new_seq_lens may be seq_lens itself. Slots behind L' in the
+ * In either case a page belongs to one sequence of the call. The pages and lengths it wrote may be read by a decode launch
+ * right behind it, rl_attention_set_prologue_overlap or not. new_seq_lens may be seq_lens itself. Slots behind L' in the
  * last destination page keep what they hold. Cached keys keep the rotation of their old positions: the caller goes on
  * counting positions for RoPE apart from cache slots. head_dim a multiple of 8 up to 1024; the pool slice and weights
  * 16-byte aligned. One call enqueues two kernels.

@@ -86,6 +86,10 @@ __device__ __forceinline__ void DependentLaunchGate() {
 // First-use set-up of the decode linear kernel on the current device (shared-memory opt-in, driver
 // entry point, error flag); rl_kernels_init calls it so that no launcher does set-up inside a capture.
 int DecodeLinearInit();
+// The same of the window attention, prompt-chunk attention and eviction kernels.
+int WindowAttentionInit();
+int PrefillAttentionInit();
+int KvEvictInit();
 
 inline bool Aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0; }
 

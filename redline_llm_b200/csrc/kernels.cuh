@@ -23,6 +23,7 @@
 // ones (LaunchKvGather, LaunchPrefillSoftmax).
 #pragma once
 
+#include <cstddef>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -173,6 +174,57 @@ inline void LaunchQkvRopeKvScatter(half* qkv, std::int64_t qkv_row_stride, const
                                               block_table_row_stride, positions, num_q_heads, num_kv_heads,
                                               head_dim, rope_theta, stream),
                 "LaunchQkvRopeKvScatter");
+}
+
+// Bounded cache (include/redline_kernels.h): attention over sinks and a sliding window, decode attention that accumulates
+// each cached token's weight, and eviction by it. Workspaces: rl_window_attention_workspace_bytes and
+// rl_window_prefill_workspace_bytes, zeroed once.
+inline void LaunchPagedWindowAttentionDecode(half* out, std::int64_t out_row_stride, const half* q, std::int64_t q_row_stride,
+                                             const half* kv_pool_layer, const std::int32_t* block_tables,
+                                             const std::int32_t* seq_lens, std::int32_t num_seqs,
+                                             std::int32_t max_blocks_per_seq, std::int32_t num_q_heads,
+                                             std::int32_t num_kv_heads, std::int32_t head_dim, float scale, std::int32_t window,
+                                             std::int32_t sinks, void* workspace, std::size_t workspace_bytes,
+                                             cudaStream_t stream) {
+  detail::Check(rl_launch_paged_window_attention_decode(out, out_row_stride, q, q_row_stride, kv_pool_layer, block_tables,
+                                                        seq_lens, num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads,
+                                                        head_dim, scale, window, sinks, workspace, workspace_bytes, stream),
+                "LaunchPagedWindowAttentionDecode");
+}
+
+inline void LaunchPagedAttentionDecodeWeights(half* out, std::int64_t out_row_stride, const half* q, std::int64_t q_row_stride,
+                                              const half* kv_pool_layer, const std::int32_t* block_tables,
+                                              const std::int32_t* seq_lens, std::int32_t num_seqs,
+                                              std::int32_t max_blocks_per_seq, std::int32_t num_q_heads,
+                                              std::int32_t num_kv_heads, std::int32_t head_dim, float scale, float* weights,
+                                              void* workspace, std::size_t workspace_bytes, cudaStream_t stream) {
+  detail::Check(rl_launch_paged_attention_decode_weights(out, out_row_stride, q, q_row_stride, kv_pool_layer, block_tables,
+                                                         seq_lens, num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads,
+                                                         head_dim, scale, weights, workspace, workspace_bytes, stream),
+                "LaunchPagedAttentionDecodeWeights");
+}
+
+inline void LaunchPagedWindowPrefillAttention(half* out, std::int64_t out_row_stride, const half* q, std::int64_t q_row_stride,
+                                              const half* kv_pool_layer, const std::int32_t* block_table_row,
+                                              std::int32_t max_blocks_per_seq, std::int32_t chunk_start,
+                                              std::int32_t chunk_len, std::int32_t num_q_heads, std::int32_t num_kv_heads,
+                                              std::int32_t head_dim, float scale, std::int32_t window, std::int32_t sinks,
+                                              void* workspace, std::size_t workspace_bytes, cudaStream_t stream) {
+  detail::Check(rl_launch_paged_window_prefill_attention(out, out_row_stride, q, q_row_stride, kv_pool_layer, block_table_row,
+                                                         max_blocks_per_seq, chunk_start, chunk_len, num_q_heads, num_kv_heads,
+                                                         head_dim, scale, window, sinks, workspace, workspace_bytes, stream),
+                "LaunchPagedWindowPrefillAttention");
+}
+
+inline void LaunchKvEvict(half* kv_pool_layer, float* weights, const std::int32_t* block_tables,
+                          std::int32_t max_blocks_per_seq, const std::int32_t* dst_block_tables,
+                          std::int32_t dst_max_blocks_per_seq, const std::int32_t* seq_lens, std::int32_t* new_seq_lens,
+                          std::int32_t* kept, std::int32_t num_seqs, std::int32_t num_kv_heads, std::int32_t head_dim,
+                          std::int32_t budget, std::int32_t sinks, std::int32_t recent, cudaStream_t stream) {
+  detail::Check(rl_launch_kv_evict(kv_pool_layer, weights, block_tables, max_blocks_per_seq, dst_block_tables,
+                                   dst_max_blocks_per_seq, seq_lens, new_seq_lens, kept, num_seqs, num_kv_heads, head_dim,
+                                   budget, sinks, recent, stream),
+                "LaunchKvEvict");
 }
 
 }  // namespace redline::kernels

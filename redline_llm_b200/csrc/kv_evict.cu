@@ -395,7 +395,6 @@ constexpr int kCluster = 8;
 // kLookup: rows a warp looks up at a time; in place (the K = 128 form) also the rows it has in registers at a time.
 template <bool kInPlace, int kRowWords, int kLookup, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, kWarps > kMoveWarps ? 1 : 4) MoveKernel(const Params p, int parts) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int seq = blockIdx.x / parts, part = blockIdx.x % parts, head = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -480,6 +479,9 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps > kMoveWarps ? 1 : 4) Move
     }
     if (moves) p.weights[weight_to] = weight;
   }
+  // Not released early: a decode launch behind this one may, under the overlap option, request pages and read lengths
+  // before its own wait. It starts when every block here has ended, and by then these writes are done.
+  __threadfence();
 }
 
 // First use on a device: the selection's shared memory.
@@ -497,6 +499,7 @@ int EnsureReady(const char* fn) {
 }
 
 }  // namespace evict
+int KvEvictInit() { return evict::EnsureReady("kv_evict"); }
 }  // namespace rl
 
 extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int32_t* block_tables,
@@ -525,7 +528,7 @@ extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int
     return Fail(RL_E_BAD_SHAPE, "%s: in place, both tables have the same row length", fn);
   if (!Aligned16(kv_pool_layer) || !Aligned16(weights))
     return Fail(RL_E_BAD_SHAPE, "%s: the pool slice and the weights must be 16-byte aligned", fn);
-  if (num_seqs > INT32_MAX / kCluster) return Fail(RL_E_TOO_LARGE, "%s: too many sequences", fn);
+  if (num_seqs > INT32_MAX / kCluster || budget > (1 << 30)) return Fail(RL_E_TOO_LARGE, "%s: at most 2^28 sequences and a budget of 2^30", fn);
   const int64_t tokens = static_cast<int64_t>(max_blocks_per_seq) * kKvBlock;
   Params p;
   p.pool = static_cast<half*>(kv_pool_layer);

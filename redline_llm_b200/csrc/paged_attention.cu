@@ -919,8 +919,11 @@ extern "C" int rl_kernels_init(int device) {
   }
   rl::CurrentDeviceFacts();
   rl::attn::DeviceState* st;
-  const int rc = rl::attn::EnsureReady(&st);
-  return rc != RL_OK ? rc : rl::DecodeLinearInit();
+  int rc = rl::attn::EnsureReady(&st);
+  if (rc == RL_OK) rc = rl::DecodeLinearInit();
+  if (rc == RL_OK) rc = rl::WindowAttentionInit();
+  if (rc == RL_OK) rc = rl::PrefillAttentionInit();
+  return rc != RL_OK ? rc : rl::KvEvictInit();
 }
 
 #ifdef RL_ATTN_TIMELINE

@@ -1065,6 +1065,10 @@ int LaunchChunk(const char* fn, void* out, int64_t out_row_stride, const void* q
 }
 
 }  // namespace pfa
+int PrefillAttentionInit() {
+  pfa::DeviceState* st;
+  return pfa::EnsureReady(&st);
+}
 }  // namespace rl
 
 extern "C" int rl_launch_paged_prefill_attention(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,

@@ -7,10 +7,11 @@
 // What bounds it: each visible K and V row is read once and used for 1 to 8 queries, far below the tensor cores' need,
 // so the kernel is a stream over pages and everything is arranged for bytes in flight:
 //  * The visible pages of all (sequence, KV head) items - sink pages, then window pages, as one list per item - are laid
-//    end to end and cut into one equal share per CTA, one persistent CTA per SM (fewer when there are fewer than eight
-//    pages for each: a page per warp is the finest useful cut). Eight warps walk a share page by page, each with its own
-//    ring of three 8 KiB stages (K tile and V tile of a page in one TMA copy, 128-byte swizzled): 192 KB in flight
-//    per SM, more than latency x bandwidth asks for.
+//    end to end and cut into one equal share per CTA, one persistent CTA per SM; few items are cut into chunks with a CTA
+//    each instead. Eight warps walk a share page by page, each with its own ring of three 8 KiB stages (K tile and V tile
+//    of a page in one TMA copy, 128-byte swizzled): 192 KB in flight per SM, more than latency x bandwidth asks for.
+//    64 sequences with a window of 4096 and 16 sinks: 45.4 us, 5.7 TB/s. What is left around the stream is a chain of
+//    ~6 us - lengths, table, first pages; fold, record, ticket, merge - which is all there is to a small call (300 tokens: 6.3 us).
 //  * S^T = K.Q^T and O^T = V^T.P^T on mma.sync m16n8k16: 16 tokens of a page fill M, the group's queries fill N = 8.
 //    The online softmax keeps FP32 maxima and sums; probabilities go to FP16 for P.V (relative 2^-12 on average, the
 //    size of the output's own rounding), their sum is taken before that rounding.
@@ -759,6 +760,12 @@ struct Call {
   cudaStream_t stream;
 };
 
+// Pages that a row can see at most.
+int64_t LongestList(const Call& c) {
+  const int64_t list = (static_cast<int64_t>(c.sinks) + kKvBlock - 1) / kKvBlock + (static_cast<int64_t>(c.window) + kKvBlock - 2) / kKvBlock + 1;
+  return list < c.max_blocks ? list : c.max_blocks;
+}
+
 int Check(const Call& c, bool with_weights) {
   if (!c.out || !c.q || !c.pool || !c.tables || !c.seq_lens || !c.workspace || (with_weights && !c.weights))
     return Fail(RL_E_NULL_POINTER, "%s: null device pointer", c.fn);
@@ -771,6 +778,9 @@ int Check(const Call& c, bool with_weights) {
   if (!(c.scale > 0.0f) || !(c.scale * 1.4426950408889634f <= 3.402823466e38f))
     return Fail(RL_E_BAD_SHAPE, "%s: scale must be positive and finite", c.fn);
   if (c.window < 1 || c.sinks < 0) return Fail(RL_E_BAD_SHAPE, "%s: window >= 1 and sinks >= 0", c.fn);
+  const int64_t rows = c.num_seqs < kMaxSeqsPerLaunch ? c.num_seqs : kMaxSeqsPerLaunch;
+  if (LongestList(c) * rows * c.kv_heads > INT32_MAX - 65536)
+    return Fail(RL_E_TOO_LARGE, "%s: more than 2^31 pages (times KV heads) in one launch", c.fn);
   if (!Aligned16(c.pool)) return Fail(RL_E_BAD_SHAPE, "%s: the pool slice must be 16-byte aligned", c.fn);
   if ((c.q_row_stride & 1) || (reinterpret_cast<uintptr_t>(c.q) & 3)) return Fail(RL_E_BAD_SHAPE, "%s: q rows must be 4-byte aligned", c.fn);
   if ((reinterpret_cast<uintptr_t>(c.out) & 1) || (reinterpret_cast<uintptr_t>(c.weights) & 3) || !Aligned16(c.workspace))
@@ -806,12 +816,7 @@ int Launch(const Call& c) {
   float* scores = reinterpret_cast<float*>(ws + kMetaBytes + kRecordBytes + StatsBytes(c.num_seqs, c.q_heads));
   p.run_ahead = g_launch_overlap;
   p.wide_out = (reinterpret_cast<uintptr_t>(c.out) & 7) == 0 && (c.out_row_stride & 3) == 0;
-  // No more CTAs than shares of kMinPagesPerCta pages can exist: a row's list is at most this long.
-  const int64_t list = p.sink_pages + ((p.window + kKvBlock - 2) >> kKvBlockShift) + 1;
-  const int64_t pages = list < c.max_blocks ? list : c.max_blocks;
-  const int64_t rows = c.num_seqs < kMaxSeqsPerLaunch ? c.num_seqs : kMaxSeqsPerLaunch;
-  if (pages * rows * c.kv_heads > INT32_MAX - 65536)
-    return Fail(RL_E_TOO_LARGE, "%s: more than 2^31 pages (times KV heads) in one launch", c.fn);
+  const int64_t pages = LongestList(c);   // no more CTAs than shares of kMinPagesPerCta pages can exist
   const int sms = CurrentDeviceFacts().sm_count < kMaxCtas ? CurrentDeviceFacts().sm_count : kMaxCtas;
   const int64_t row = static_cast<int64_t>(c.q_heads) * c.max_blocks * kKvBlock;
   for (int first = 0; first < c.num_seqs; first += kMaxSeqsPerLaunch) {
@@ -847,6 +852,7 @@ int Launch(const Call& c) {
 }
 
 }  // namespace wattn
+int WindowAttentionInit() { return wattn::EnsureReady("window attention"); }
 }  // namespace rl
 
 extern "C" int rl_window_attention_workspace_bytes(int32_t num_seqs, int32_t max_blocks_per_seq, int32_t num_q_heads,

@@ -228,6 +228,16 @@ def launch_paged_prefill_attention(out, out_row_stride, q, q_row_stride, kv_pool
         "paged prefill attention")
 
 
+def _here(*tensors) -> None:
+    """The bounded-cache launchers' own check: a tensor of another device than the current one (or of the host) would
+    reach the kernel as a pointer it may not touch."""
+    import torch
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"a tensor on {t.device} was given to a launch on cuda:{here}")
+
+
 def _workspace(bytes_needed: int, device):
     import torch
     return torch.zeros(max(16, bytes_needed), dtype=torch.uint8, device="cuda" if device is None else device)
@@ -260,6 +270,7 @@ def launch_paged_window_attention_decode(out, out_row_stride, q, q_row_stride, k
                                          window, sinks, workspace, stream=None, q_offset=0):
     """launch_paged_attention_decode over the first `sinks` and the last `window` cached tokens of each sequence;
     pages (and table entries) outside both are not read. 1 to 8 query heads per KV head."""
+    _here(out, q, kv_pool_layer, block_tables, seq_lens, workspace)
     _check(lib().rl_launch_paged_window_attention_decode(
         _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_tables.data_ptr(),
         seq_lens.data_ptr(), num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads, head_dim, scale, window, sinks,
@@ -272,6 +283,7 @@ def launch_paged_attention_decode_weights(out, out_row_stride, q, q_row_stride, 
     """Decode attention over the whole cache that adds each cached token's softmax probabilities, summed over the
     query heads of a group, to weights (float32 [num_blocks, num_kv_heads, 16], paged like the pool); the newest
     token's entry is set, not added to."""
+    _here(out, q, kv_pool_layer, block_tables, seq_lens, weights, workspace)
     _check(lib().rl_launch_paged_attention_decode_weights(
         _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_tables.data_ptr(),
         seq_lens.data_ptr(), num_seqs, max_blocks_per_seq, num_q_heads, num_kv_heads, head_dim, scale, _ptr(weights),
@@ -295,6 +307,7 @@ def launch_paged_window_prefill_attention(out, out_row_stride, q, q_row_stride, 
                                           head_dim, scale, window, sinks, workspace=None, stream=None, q_offset=0):
     """launch_paged_prefill_attention with a sliding window and sinks: row i sees the first `sinks` tokens and the
     last `window` up to its own position. Without a workspace no work is cut across CTAs (slower, same function)."""
+    _here(out, q, kv_pool_layer, block_table_row, workspace)
     _check(lib().rl_launch_paged_window_prefill_attention(
         _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_table_row.data_ptr(),
         max_blocks_per_seq, chunk_start, chunk_len, num_q_heads, num_kv_heads, head_dim, scale, window, sinks,
@@ -307,6 +320,7 @@ def launch_kv_evict(kv_pool_layer, weights, block_tables, max_blocks_per_seq, ds
     """Shrinks each sequence's cache to `budget` tokens per KV head: the first `sinks`, the last `recent` and the
     heaviest of the rest, moved in cache order to the pages of dst_block_tables (the same tensor as block_tables: in
     place). kept (int32 [num_seqs, num_kv_heads, budget]) receives the slots they had, -1 behind the last."""
+    _here(kv_pool_layer, weights, block_tables, dst_block_tables, seq_lens, new_seq_lens, kept)
     _check(lib().rl_launch_kv_evict(
         _ptr(kv_pool_layer), _ptr(weights), block_tables.data_ptr(), max_blocks_per_seq, dst_block_tables.data_ptr(),
         dst_max_blocks_per_seq, seq_lens.data_ptr(), new_seq_lens.data_ptr(), kept.data_ptr(), num_seqs, num_kv_heads,

@@ -72,6 +72,7 @@ def test_refusals_of_one_launcher_only():
         assert call(qs=2047) == SHAPE and call(q=P + 2) == SHAPE and call(ws=P + 8) == SHAPE
         assert call(mb=(1 << 26) + 1) == LARGE
         assert call(wb=0) == WORKSPACE
+        assert call(**dict(dict(mb=1 << 26, n=64, wb=(1 << 64) - 1), **(dict(window=2**31 - 1) if call is decode else {}))) == LARGE
         need = K.window_attention_workspace_bytes(4, 8, 12, 2, weights=call is weights)
         assert call(wb=need - 1) == WORKSPACE and b"workspace" in K.lib().rl_last_error()
         assert call(n=0, out=None) == 0 and call(n=-3, out=None) == 0
@@ -92,6 +93,7 @@ def test_evict_refusals():
                    dict(budget=0), dict(budget=-1), dict(sinks=-1), dict(recent=-1), dict(sinks=60, recent=5),
                    dict(sinks=2**31 - 1, recent=2**31 - 1), dict(budget=65), dict(dst=P), dict(pool=P + 8), dict(w=P + 2)):
         assert evict(**change) == SHAPE, change
+    assert evict(budget=(1 << 30) + 1, mb=1 << 26, dmb=1 << 26) == LARGE and evict(n=1 << 28) == LARGE
     assert evict(mb=(1 << 26) + 1) == LARGE and evict(dmb=(1 << 26) + 1) == LARGE
     assert evict(n=0, pool=None) == 0 and evict(n=-1, pool=None) == 0
 

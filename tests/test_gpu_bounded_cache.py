@@ -280,6 +280,7 @@ def test_window_prefill_cut_across_ctas(start, rows, window, sinks):
     c = Cache([start + rows], 2, seed=rows)
     q, out, qs, os_ = decode_case_rows(c, rows, 12, 1536, 1536)
     whole, again = out.clone(), out.clone()
+    assert rows == 3000 or K.window_prefill_workspace_bytes(start, rows, 12, window, sinks) > 0
     run_prefill(c, q, out, qs, os_, start, rows, 12, window, sinks)
     run_prefill(c, q, again, qs, os_, start, rows, 12, window, sinks)
     run_prefill(c, q, whole, qs, os_, start, rows, 12, window, sinks, ws=None)
@@ -399,6 +400,11 @@ def some_weights(c, kind):
         return (u * 4).floor()
     if kind == "equal":
         return torch.full_like(u, 0.25)
+    if kind == "crowded":                    # nearly all in one part in two thousand of the range, many of them equal
+        w = 1.0 + (u * 500).floor() * 1e-6
+        w[u < 0.002] = 1e30
+        w[(u > 0.5) & (u < 0.501)] = -1e30
+        return w
     if kind == "odd":
         w = u - 0.5
         w[u < 0.2] = float("nan")
@@ -427,6 +433,21 @@ def test_evict(budget, sinks, recent, kind, in_place):
 def test_evict_sizes(lens, kv, budget, sinks, recent, in_place):
     c = Cache(lens, kv, seed=kv, extra_pages=len(lens) * ((budget + 15) // 16), head_dim=D)
     check_evict(c, budget, sinks, recent, some_weights(c, "spread"), in_place)
+
+
+@pytest.mark.parametrize("lens,kv,budget", [([6000, 3000], 1, 1500), ([9000] * 40, 2, 4000), ([30000], 2, 9000)])
+def test_evict_weights_that_share_a_bin(lens, kv, budget):
+    """Thousands of candidates fall into one bin of the first division, with and without a cluster per item."""
+    c = Cache(lens, kv, seed=kv + 7)
+    check_evict(c, budget, 4, 100, some_weights(c, "crowded"), True)
+
+
+def test_evict_more_tokens_than_shared_memory_holds():
+    """80 items, so one CTA each, two of them longer than the keys that a CTA keeps."""
+    c = Cache([47001, 50] + [100] * 8, 8, seed=12)
+    check_evict(c, 700, 4, 20, some_weights(c, "spread"), True)
+    c = Cache([47001, 50] + [100] * 8, 8, seed=13)
+    check_evict(c, 40000, 0, 0, some_weights(c, "ties"), True)
 
 
 @pytest.mark.parametrize("head_dim", [8, 64, 96, 256, 1024])
@@ -524,6 +545,132 @@ def test_streams_with_a_workspace_each():
     for c, (q, out, _, _), (pq, pout, _, _) in zip(cases, io, pf):
         check_decode(c, q, out, 12, 1000, 4)
         check_prefill(c, pq, pout, 700, 200, 12, 600, 4, some=[0, 100, 199])
+
+
+@pytest.mark.parametrize("shift,stride", [(0, 1537), (1, 1538), (2, 1540), (4, 1540)])
+def test_decode_output_rows_of_any_alignment(shift, stride):
+    c = Cache([700, 90], 2, seed=70)
+    q, _, qs, _ = decode_case(c, 12, 0, 0, 0)
+    buf = torch.full((3 * stride + 8,), 7.0, dtype=torch.float16, device="cuda")
+    out = buf[shift:shift + 3 * stride].view(3, stride)
+    ws = K.window_attention_workspace(2, c.mbps, 12, 2)
+    K.launch_paged_window_attention_decode(out, stride, q, qs, c.pool, c.tables, c.seq_lens, 2, c.mbps, 12, 2, D, SCALE, 300, 4, ws)
+    check_decode(c, q, out, 12, 300, 4)
+    assert bool((buf[:shift] == 7.0).all()) and bool((buf[shift + 3 * stride:] == 7.0).all())
+
+
+def test_tensors_elsewhere_are_refused():
+    c = Cache([40], 2, seed=71)
+    q, out, qs, os_ = decode_case(c, 12, 0, 0, 0)
+    ws = K.window_attention_workspace(1, c.mbps, 12, 2, weights=True)
+    w = torch.zeros(c.blocks, 2, PAGE, device="cuda")
+    kept = torch.zeros(1, 2, 16, dtype=torch.int32, device="cuda")
+    with pytest.raises(K.KernelError):
+        K.launch_paged_window_attention_decode(out, os_, q.cpu(), qs, c.pool, c.tables, c.seq_lens, 1, c.mbps, 12, 2, D, SCALE, 9, 0, ws)
+    with pytest.raises(K.KernelError):
+        K.launch_paged_attention_decode_weights(out, os_, q, qs, c.pool, c.tables, c.seq_lens.cpu(), 1, c.mbps, 12, 2, D, SCALE, w, ws)
+    with pytest.raises(K.KernelError):
+        K.launch_paged_window_prefill_attention(out, os_, q, qs, c.pool, c.tables.cpu(), c.mbps, 39, 1, 12, 2, D, SCALE, 9, 0, None)
+    with pytest.raises(K.KernelError):
+        K.launch_kv_evict(c.pool, w.cpu(), c.tables, c.mbps, c.tables, c.mbps, c.seq_lens, c.seq_lens, kept, 1, 2, D, 16, 0, 0)
+    assert bool((out == 7.0).all())
+
+
+def test_prompt_attention_and_eviction_in_graphs():
+    """Captured and replayed: a chunk cut into runs, and an eviction to other pages; the same bits as when launched."""
+    c = Cache([9000], 2, seed=72, extra_pages=80)
+    pq, pout, pqs, pos_ = decode_case_rows(c, 64, 12, 1536, 1536)
+    pws = K.window_prefill_workspace(8936, 64, 12, 6000, 20)
+    assert K.window_prefill_workspace_bytes(8936, 64, 12, 6000, 20) > 0, "this chunk is meant to be cut"
+    w = some_weights(c, "spread")
+    dst = c.free[:63].view(1, 63).int().contiguous()
+    new = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kept = torch.zeros(1, 2, 1000, dtype=torch.int32, device="cuda")
+
+    def go():
+        run_prefill(c, pq, pout, pqs, pos_, 8936, 64, 12, 6000, 20, ws=pws)
+        K.launch_kv_evict(c.pool, w, c.tables, c.mbps, dst, 63, c.seq_lens, new, kept, 1, 2, D, 1000, 4, 100)
+
+    go()
+    want = [x.clone() for x in (pout, c.pool.view(torch.int16), w.view(torch.int32), new, kept)]
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        go()
+    pout.fill_(7.0)
+    new.zero_()
+    kept.zero_()
+    c.pool[dst[0].long()] = 0
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert bool((pout[:64] == want[0][:64]).all()) and torch.equal(new, want[3]) and torch.equal(kept, want[4])
+    live = torch.arange(1000, device="cuda")
+    b, sl = dst[0].long()[live // PAGE], live % PAGE
+    assert torch.equal(c.pool.view(torch.int16)[b, :, :, sl], want[1][b, :, :, sl])
+    assert torch.equal(w.view(torch.int32), want[2])
+
+
+def test_with_dependent_launch_on_a_step_sees_what_the_launches_before_it_wrote():
+    """rl_attention_set_prologue_overlap: scatter, weights, window attention and an eviction in place back to back, launched
+    many times without a pause, and in a graph - the same bits as with the option off."""
+    def loop(overlap, graph):
+        K.set_attention_prologue_overlap(overlap)
+        try:
+            c = Cache([900, 1500, 64], 2, seed=80)
+            g = torch.Generator(device="cuda")
+            g.manual_seed(81)
+            rows, heads, kv = 3, 12, 2
+            fresh = [torch.randn(rows, kv * D, generator=g, device="cuda").half() for _ in range(12)]
+            q = torch.randn(rows, heads * D, generator=g, device="cuda").half()
+            w = torch.rand(c.blocks, kv, PAGE, generator=g, device="cuda")
+            outs = [torch.zeros(rows, heads * D, dtype=torch.float16, device="cuda") for _ in range(18)]
+            kept = torch.zeros(rows, kv, 800, dtype=torch.int32, device="cuda")
+            ws = K.window_attention_workspace(rows, c.mbps, heads, kv, weights=True)
+            lens0, pool0, w0 = c.seq_lens.clone(), c.pool.clone(), w.clone()
+            pos = c.seq_lens - 1
+
+            def go():
+                for i in range(6):
+                    K.launch_kv_scatter(c.pool, fresh[2 * i], fresh[2 * i + 1], kv * D, kv * D, c.tables, c.mbps, pos, rows, kv, D)
+                    K.launch_paged_attention_decode_weights(outs[3 * i], heads * D, q, heads * D, c.pool, c.tables, c.seq_lens, rows,
+                                                            c.mbps, heads, kv, D, SCALE, w, ws)
+                    K.launch_paged_window_attention_decode(outs[3 * i + 1], heads * D, q, heads * D, c.pool, c.tables, c.seq_lens,
+                                                           rows, c.mbps, heads, kv, D, SCALE, 200, 4, ws)
+                    if i == 2:
+                        K.launch_kv_evict(c.pool, w, c.tables, c.mbps, c.tables, c.mbps, c.seq_lens, c.seq_lens, kept, rows, kv, D,
+                                          800, 4, 100)
+                    K.launch_paged_window_attention_decode(outs[3 * i + 2], heads * D, q, heads * D, c.pool, c.tables, c.seq_lens,
+                                                           rows, c.mbps, heads, kv, D, SCALE, 10000, 0, ws)
+                    pos.copy_(c.seq_lens - 1)
+
+            torch.cuda.synchronize()
+            if graph:
+                go()
+                torch.cuda.synchronize()
+                cg = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(cg):
+                    go()
+                run = cg.replay
+            else:
+                run = go
+            for _ in range(5):
+                c.seq_lens.copy_(lens0)
+                c.pool.view(torch.int16).copy_(pool0.view(torch.int16))
+                w.copy_(w0)
+                pos.copy_(lens0 - 1)
+                torch.cuda.synchronize()
+                run()
+                torch.cuda.synchronize()
+                yield [x.clone() for x in outs] + [c.pool.view(torch.int16).clone(), w.view(torch.int32).clone(), c.seq_lens.clone(), kept.clone()]
+        finally:
+            K.set_attention_prologue_overlap(False)
+
+    want = next(iter(loop(False, False)))
+    for overlap, graph in ((False, True), (True, False), (True, True)):
+        for got in loop(overlap, graph):
+            for a, b in zip(want, got):
+                assert torch.equal(a.nan_to_num(7.0) if a.is_floating_point() else a, b.nan_to_num(7.0) if b.is_floating_point() else b)
 
 
 def test_a_request_with_a_bounded_cache():
