@@ -50,20 +50,17 @@ __device__ __forceinline__ int CachedTokens(const Params& p, int seq) {
   return max(0, min(p.seq_lens[seq], p.max_blocks * kKvBlock));
 }
 
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kMaxSelectCluster = 8;
 constexpr int kBinBits = 11, kBins = 1 << kBinBits;
-constexpr int kListed = 1024;      // candidates of a bin that are taken out of the crowd: one per thread
+constexpr int kMaxListed = 1024;   // candidates of a bin that are taken out of the crowd: one per thread
 constexpr int kRanked = 64;        // of those, as many as are simply ranked against one another
 constexpr int kLoadAhead = 8;      // quads of weights a thread has in flight
 constexpr int kMaxCachedKeys = 45 * 1024;   // 180 KB
-static_assert(kBins == 2 * kSelectThreads && kListed <= kSelectThreads, "two bins per thread, a thread per listed key");
 
 // What the CTAs of a cluster tell one another.
 struct Shared {
   int bins[kBins];
-  uint32_t list[kListed];
+  uint32_t list[kMaxListed];
   uint32_t lo, hi;       // range of this CTA's keys
   int listed;            // keys in its list
   int sure, equal;       // its tokens above the threshold (or kept in any case), and at it
@@ -89,8 +86,12 @@ __device__ __forceinline__ int2 LoadPeer2(const int* mine, int rank) {   // two 
   return v;
 }
 
-// Grid: (sequences * cluster, KV heads). CTA `rank` of an item's cluster has every quad of tokens of its slice.
-__global__ void __launch_bounds__(kSelectThreads, 1) SelectKernel(const Params p, int cluster) {
+// Grid: (sequences * cluster, KV heads). CTA `rank` of an item's cluster has every quad of tokens of its slice. 1024 threads
+// where a CTA has its SM to itself; 512, without clusters, where there are more items than SMs and CTAs share one.
+template <int kSelectThreads>
+__global__ void __launch_bounds__(kSelectThreads, 1024 / kSelectThreads) SelectKernel(const Params p, int cluster) {
+  constexpr int kSelectWarps = kSelectThreads / 32, kListed = kSelectThreads, kPerThread = kBins / kSelectThreads;
+  static_assert(kListed <= kMaxListed && kPerThread % 2 == 0, "a thread per listed key, pairs of bins");
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ __align__(16) Shared sh;
   __shared__ __align__(16) uint32_t crowd[kListed + 4];
@@ -139,7 +140,10 @@ __global__ void __launch_bounds__(kSelectThreads, 1) SelectKernel(const Params p
 #pragma unroll 4
     for (int q = q_first + tid; q < q_last; q += kSelectThreads) use_quad(q, quad(q), use);
   };
-  auto clear_bins = [&](int* bins) { bins[tid] = bins[tid + kSelectThreads] = 0; };
+  auto clear_bins = [&](int* bins) {
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) bins[tid + i * kSelectThreads] = 0;
+  };
 
   // thr: tokens with a larger key stay, and the first `ties` of those whose key equals it
   uint32_t thr = 0xFFFFFFFFu;   // no weight has this key
@@ -180,8 +184,8 @@ __global__ void __launch_bounds__(kSelectThreads, 1) SelectKernel(const Params p
       warp_hi[warp] = hi;
     }
     __syncthreads();
-    lo = __reduce_min_sync(0xffffffffu, warp_lo[lane]);
-    hi = __reduce_max_sync(0xffffffffu, warp_hi[lane]);
+    lo = __reduce_min_sync(0xffffffffu, warp_lo[lane % kSelectWarps]);
+    hi = __reduce_max_sync(0xffffffffu, warp_hi[lane % kSelectWarps]);
     if (cluster > 1) {
       if (tid == 0) {
         sh.lo = lo;
@@ -198,36 +202,44 @@ __global__ void __launch_bounds__(kSelectThreads, 1) SelectKernel(const Params p
 #pragma unroll 1
     while (true) {
       const int shift = max(0, 32 - __clz(hi - lo) - kBinBits);
-      int upper_bin, lower_bin;   // of thread i: bins 2047 - 2i and 2046 - 2i, from the top down
+      int bin[kPerThread];   // this thread's bins, from the top down: bin[i] is number top - i
+      const int top = kBins - 1 - kPerThread * tid;
       if (count == 0) {
         for_each([&](uint32_t k) {
           if (k >= lo && k <= hi) atomicAdd(&sh.bins[(k - lo) >> shift], 1);
         });
-        upper_bin = lower_bin = 0;
         if (cluster > 1) {
           ClusterBarrier();
-          int2 pair[kMaxSelectCluster];   // all requests under way before the first is used
+          static_assert(kMaxSelectCluster == 8, "unrolled below");
 #pragma unroll
-          for (int r = 0; r < kMaxSelectCluster; ++r) pair[r] = r < cluster ? LoadPeer2(&sh.bins[kBins - 2 - 2 * tid], r) : make_int2(0, 0);
+          for (int i = 0; i < kPerThread; i += 2) {
+            int2 pair[kMaxSelectCluster];   // all requests under way before the first is used
 #pragma unroll
-          for (int r = 0; r < kMaxSelectCluster; ++r) {
-            upper_bin += pair[r].y;
-            lower_bin += pair[r].x;
+            for (int r = 0; r < kMaxSelectCluster; ++r) pair[r] = r < cluster ? LoadPeer2(&sh.bins[top - i - 1], r) : make_int2(0, 0);
+            bin[i] = bin[i + 1] = 0;
+#pragma unroll
+            for (int r = 0; r < kMaxSelectCluster; ++r) {
+              bin[i] += pair[r].y;
+              bin[i + 1] += pair[r].x;
+            }
           }
         } else {
           __syncthreads();
-          upper_bin = sh.bins[kBins - 1 - 2 * tid];
-          lower_bin = sh.bins[kBins - 2 - 2 * tid];
+#pragma unroll
+          for (int i = 0; i < kPerThread; ++i) bin[i] = sh.bins[top - i];
         }
       } else {
         clear_bins(local_bins);
         __syncthreads();
         if (tid < count && mine >= lo && mine <= hi) atomicAdd(&local_bins[(mine - lo) >> shift], 1);
         __syncthreads();
-        upper_bin = local_bins[kBins - 1 - 2 * tid];
-        lower_bin = local_bins[kBins - 2 - 2 * tid];
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) bin[i] = local_bins[top - i];
       }
-      int incl = upper_bin + lower_bin;
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < kPerThread; ++i) sum += bin[i];
+      int incl = sum;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, off);
@@ -235,12 +247,15 @@ __global__ void __launch_bounds__(kSelectThreads, 1) SelectKernel(const Params p
       }
       if (lane == 31) warp_sum[warp] = incl;
       __syncthreads();
-      const int above = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0) + incl - upper_bin - lower_bin;
-      if (above < need && above + upper_bin + lower_bin >= need) {
-        const bool upper = above + upper_bin >= need;
-        found_bin = kBins - 1 - 2 * tid - (upper ? 0 : 1);
-        found_above = above + (upper ? 0 : upper_bin);
-        found_count = upper ? upper_bin : lower_bin;
+      int above = __reduce_add_sync(0xffffffffu, lane < warp && lane < kSelectWarps ? warp_sum[lane] : 0) + incl - sum;
+#pragma unroll
+      for (int i = 0; i < kPerThread; ++i) {
+        if (above < need && above + bin[i] >= need) {   // one bin of one thread
+          found_bin = top - i;
+          found_above = above;
+          found_count = bin[i];
+        }
+        above += bin[i];
       }
       __syncthreads();
       need -= found_above;
@@ -492,7 +507,8 @@ int EnsureReady(const char* fn) {
   bool& ready = g_ready[CurrentDeviceIndex()];
   std::lock_guard<std::mutex> lock(g_mutex);
   if (ready) return RL_OK;
-  const cudaError_t e = cudaFuncSetAttribute(SelectKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCachedKeys * 4);
+  cudaError_t e = cudaFuncSetAttribute(SelectKernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCachedKeys * 4);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(SelectKernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCachedKeys * 4);
   if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s: shared-memory opt-in: %s", fn, cudaGetErrorString(e));
   ready = true;
   return RL_OK;
@@ -552,11 +568,16 @@ extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // A cluster per item as far as the SMs go round and each CTA still has a few thousand tokens (as long as the table
   // says the sequences may be).
+  const int sm_count = CurrentDeviceFacts().sm_count;
   int cluster = 1;
-  while (cluster < kMaxSelectCluster && 2 * cluster * items <= CurrentDeviceFacts().sm_count && tokens / (2 * cluster) >= kSelectThreads * 2)
-    cluster *= 2;
-  cudaError_t e = LaunchDependent(SelectKernel, dim3(static_cast<unsigned>(num_seqs) * cluster, num_kv_heads), dim3(kSelectThreads),
-                                  static_cast<size_t>(p.cached_keys) * 4, cluster, s, p, cluster);
+  while (cluster < kMaxSelectCluster && 2 * cluster * items <= sm_count && tokens / (2 * cluster) >= 2048) cluster *= 2;
+  // More items than SMs: half the threads, so that several CTAs share an SM and wait for their loads side by side (57 x 8 items of
+  // 425-9779 tokens: 27.0 us with the move, with 1024 threads each 32.6).
+  const bool crowded = items > sm_count;
+  const size_t key_bytes = static_cast<size_t>(p.cached_keys) * 4;
+  const dim3 select_grid(static_cast<unsigned>(num_seqs) * cluster, num_kv_heads);
+  cudaError_t e = crowded ? LaunchDependent(SelectKernel<512>, select_grid, dim3(512), key_bytes, 1, s, p, 1)
+                          : LaunchDependent(SelectKernel<1024>, select_grid, dim3(1024), key_bytes, cluster, s, p, cluster);
   if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s: %s", fn, cudaGetErrorString(e));
   const bool in_place = dst_block_tables == block_tables;
   // Out of place a warp looks 32 rows up and moves them eight at a time - or, while all rows then still fit the machine

@@ -8,7 +8,7 @@
 // so the kernel is a stream over pages and everything is arranged for bytes in flight:
 //  * The visible pages of all (sequence, KV head) items - sink pages, then window pages, as one list per item - are laid
 //    end to end and cut into one equal share per CTA, one persistent CTA per SM; few items are cut into chunks with a CTA
-//    each instead. Eight warps walk a share page by page, each with its own ring of three 8 KiB stages (K tile and V tile
+//    each instead, and many small ones go to teams of warps whole. Eight warps walk a share page by page, each with its own ring of three 8 KiB stages (K tile and V tile
 //    of a page in one TMA copy, 128-byte swizzled): 192 KB in flight per SM, more than latency x bandwidth asks for.
 //    64 sequences with a window of 4096 and 16 sinks: 45.4 us, 5.7 TB/s. What is left around the stream is a chain of
 //    ~6 us - lengths, table, first pages; fold, record, ticket, merge - which is all there is to a small call (300 tokens: 6.3 us).
@@ -53,6 +53,7 @@ constexpr int kMinChunk = 2 * kWarps;      // an item is not cut finer than this
 constexpr int kWholeItem = 3 * kWarps;     // ... and not at all up to this: a ring holds three pages per warp, and handing over
                                            // costs 1 us (300 tokens: 6.65 us whole, 7.73 in two; 8000 tokens: 11.5 us in
                                            // chunks of 16 pages, 14.8 in chunks of 8, 11.6 in chunks of 32)
+constexpr int kTeamPages = 32;            // pages of an item that one warp of a team may take: their tile indices sit one per lane
 constexpr int kSegmentPages = 12;    // what a second item costs a CTA (fold and hand-over, 2-3 us), in pages
 constexpr int kMaxCtas = 256;
 constexpr int kNewestPageBit = 1 << 30;
@@ -141,6 +142,169 @@ __device__ __forceinline__ Cursor Locate(int t, const int* prefix, int num_seqs,
   return c;
 }
 
+// One page of an item: scores of its 16 tokens against the group's queries, online softmax, P.V. `st` is the stage that holds
+// its K and V tile, t0 the position of its first token; w0 is the first token of the window.
+struct PageOffsets {
+  uint32_t k[4], v[4];   // ldmatrix offsets of this lane inside a stage; dims 64..127 of a tile sit kHiDims further
+};
+constexpr uint32_t kHiDims = 2048;
+__device__ __forceinline__ PageOffsets MakePageOffsets(int lane) {
+  // K rows as the A operand of S^T, V transposed as the A operand of O^T
+  const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_sel = lane >> 4;
+  const int v_row = (lane & 7) + (lane >> 4) * 8, v_sel = (lane >> 3) & 1;
+  PageOffsets off;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    off.k[j] = k_row * 128 + (((2 * j + k_sel) ^ (k_row & 7)) << 4);
+    off.v[j] = kPageBytes + v_row * 128 + (((2 * j + v_sel) ^ (v_row & 7)) << 4);
+  }
+  return off;
+}
+struct Running {
+  float o[8][4];            // O^T: dims 16 i + g (+ 8) of queries 2 tig, 2 tig + 1
+  float m0, m1, l0, l1;     // of the two queries; l is this lane's share of the sum
+  __device__ __forceinline__ void Clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    m0 = m1 = -INFINITY;
+    l0 = l1 = 0.0f;
+  }
+};
+template <bool kScores>
+__device__ __forceinline__ void PageStep(const Params& p, uint32_t st, const PageOffsets& off, const uint32_t (&qb)[8][2], int t0,
+                                         int len, int w0, float* scores, int lane, Running& r) {
+  const int g = lane >> 2, tig = lane & 3;
+  // token i of the page is visible if i < end and (i < sink or i >= win); all 16 are on a page in the middle
+  const int end = len - t0, sink = p.sinks - t0, win = w0 - t0;
+  const bool full = end >= kKvBlock && (sink >= kKvBlock || win <= 0);
+
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t a[4], a2[4];
+    Ldsm4(st + off.k[j], a);
+    Ldsm4(st + off.k[j] + kHiDims, a2);
+    Mma16816(s, a, qb[j][0], qb[j][1]);
+    Mma16816(s2, a2, qb[j + 4][0], qb[j + 4][1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = (s[i] + s2[i]) * p.scale_log2e;
+  if (kScores) {   // [query][token]: the eight lanes of a query fill whole sectors
+    float* dst = scores + static_cast<int64_t>(t0) * p.group + 2 * tig * kKvBlock + g;
+    if (2 * tig < p.group) {
+      __stcg(dst, s[0]);
+      __stcg(dst + 8, s[2]);
+    }
+    if (2 * tig + 1 < p.group) {
+      __stcg(dst + kKvBlock, s[1]);
+      __stcg(dst + kKvBlock + 8, s[3]);
+    }
+  }
+  auto visible = [&](int i) { return i < end && (i < sink || i >= win); };
+  if (!full) {
+    if (!visible(g)) s[0] = s[1] = -INFINITY;
+    if (!visible(g + 8)) s[2] = s[3] = -INFINITY;
+  }
+  float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
+  if (__any_sync(0xffffffffu, mx0 > r.m0 || mx1 > r.m1)) {
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+    }
+    const float n0 = fmaxf(r.m0, mx0), n1 = fmaxf(r.m1, mx1);
+    const float a0 = Exp2(r.m0 - n0), a1 = Exp2(r.m1 - n1);
+    r.m0 = n0;
+    r.m1 = n1;
+    r.l0 *= a0;
+    r.l1 *= a1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      r.o[i][0] *= a0;
+      r.o[i][1] *= a1;
+      r.o[i][2] *= a0;
+      r.o[i][3] *= a1;
+    }
+  }
+  const float p0 = Exp2(s[0] - r.m0), p1 = Exp2(s[1] - r.m1);
+  const float p2 = Exp2(s[2] - r.m0), p3 = Exp2(s[3] - r.m1);
+  r.l0 += p0 + p2;
+  r.l1 += p1 + p3;
+  const uint32_t b0 = MovmT(PackHalf2(p0, p1)), b1 = MovmT(PackHalf2(p2, p3));
+  if (full) {
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) {
+      uint32_t a[4];
+      Ldsm4T(st + off.v[mt & 3] + (mt >> 2) * kHiDims, a);
+      Mma16816(r.o[mt], a, b0, b1);
+    }
+  } else {
+    // V rows of invisible tokens may hold NaN, and 0 * NaN would poison the sums: cleared in registers.
+    const uint32_t k01 = (visible(2 * tig) ? 0x0000FFFFu : 0u) | (visible(2 * tig + 1) ? 0xFFFF0000u : 0u);
+    const uint32_t k23 = (visible(2 * tig + 8) ? 0x0000FFFFu : 0u) | (visible(2 * tig + 9) ? 0xFFFF0000u : 0u);
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) {
+      uint32_t a[4];
+      Ldsm4T(st + off.v[mt & 3] + (mt >> 2) * kHiDims, a);
+      a[0] &= k01;
+      a[1] &= k01;
+      a[2] &= k23;
+      a[3] &= k23;
+      Mma16816(r.o[mt], a, b0, b1);
+    }
+  }
+}
+// The group's queries as the B operand of S^T: query g in column g, zeros past the group.
+__device__ __forceinline__ void LoadQueries(const Params& p, int seq, int head, int lane, uint32_t (&qb)[8][2]) {
+  const int g = lane >> 2, tig = lane & 3;
+  const half* qrow = p.q + static_cast<int64_t>(seq) * p.q_stride + (static_cast<int64_t>(head) * p.group + g) * kHeadDim + 2 * tig;
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) {
+    qb[kk][0] = g < p.group ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * kk)) : 0u;
+    qb[kk][1] = g < p.group ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * kk + 8)) : 0u;
+  }
+}
+// A warp's running sums into its part of the fold's buffer: o[query][128] (columns permuted by the query pair: no bank is
+// met twice), m and l of each query.
+__device__ __forceinline__ void LeaveInBuffer(Running& r, float* obuf, float* mbuf, float* lbuf, int warp, int lane) {
+  const int g = lane >> 2, tig = lane & 3;
+#pragma unroll
+  for (int off = 4; off < 32; off <<= 1) {
+    r.l0 += __shfl_xor_sync(0xffffffffu, r.l0, off);
+    r.l1 += __shfl_xor_sync(0xffffffffu, r.l1, off);
+  }
+  float* ob = obuf + (warp * kMaxGroup + 2 * tig) * kHeadDim;
+#pragma unroll
+  for (int mt = 0; mt < 8; ++mt) {
+    const int c0 = (16 * mt + g) ^ (tig * 8), c1 = (16 * mt + g + 8) ^ (tig * 8);
+    ob[c0] = r.o[mt][0];
+    ob[kHeadDim + c0] = r.o[mt][1];
+    ob[c1] = r.o[mt][2];
+    ob[kHeadDim + c1] = r.o[mt][3];
+  }
+  if (g == 0) {
+    mbuf[(2 * tig) * kWarps + warp] = r.m0;
+    mbuf[(2 * tig + 1) * kWarps + warp] = r.m1;
+    lbuf[(2 * tig) * kWarps + warp] = r.l0;
+    lbuf[(2 * tig + 1) * kWarps + warp] = r.l1;
+  }
+}
+// Columns 4 lane .. 4 lane + 3 of a finished row: divided by the sum, rounded once.
+template <bool kScores>
+__device__ __forceinline__ void WriteRow(const Params& p, int seq, int qh, int lane, const float4& a, float m, float l) {
+  half* dst = p.out + static_cast<int64_t>(seq) * p.out_stride + static_cast<int64_t>(qh) * kHeadDim + 4 * lane;
+  const half2 lo = __floats2half2_rn(a.x / l, a.y / l), hi = __floats2half2_rn(a.z / l, a.w / l);
+  if (p.wide_out) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(AsU32(lo), AsU32(hi));
+  } else {
+    dst[0] = __low2half(lo);
+    dst[1] = __high2half(lo);
+    dst[2] = __low2half(hi);
+    dst[3] = __high2half(hi);
+  }
+  if (kScores && lane == 0) p.stats[static_cast<int64_t>(seq) * p.kv_heads * p.group + qh] = make_float2(m, 1.0f / l);
+}
+
 template <bool kScores>
 __global__ void __launch_bounds__(kThreads, 1)
 DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
@@ -156,7 +320,6 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   __shared__ bool merge_here, others_done;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, tig = lane & 3;
   const int heads = p.kv_heads;
   if (!kScores) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == kThreads - 1) {
@@ -219,12 +382,102 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   // and 14.4 us; 64 x 1024-1280, 128 items, stay with shares.)
   int longest = 0;
   bool chunked = false;
-  if (items < static_cast<int>(gridDim.x)) {
+  if (items <= static_cast<int>(gridDim.x)) {
     const int spare = static_cast<int>(gridDim.x) - items;
-    const int fit = (total - 1) / spare + 1;   // sum of ceil(pages / fit) <= total / fit + items <= the grid
+    const int fit = spare > 0 ? (total - 1) / spare + 1 : most_pages;   // sum of ceil(pages / fit) <= total / fit + items <= the grid
     longest = max(min(fit, most_pages), kMinChunk);
     chunked = longest <= max(total / static_cast<int>(gridDim.x), kMinChunk) + kSegmentPages;
   }
+  const uint32_t my_ring = SmemAddr(smem) + warp * (kStages * kStageBytes);
+  const uint32_t my_bars = SmemAddr(smem + kBarOff) + warp * (kStages * 8);
+  const uint64_t policy = L2PolicyEvictFirst();   // pages are read once per launch
+  const PageOffsets off = MakePageOffsets(lane);
+  bool failed = false;
+  int fail_at = 0;
+  auto request = [&](int stage, int tile) {
+    if (lane == 0) {
+      MbarExpectTx(my_bars + stage * 8, kStageBytes);
+      TmaLoadPage(my_ring + stage * kStageBytes, &tile_map, tile & ~kNewestPageBit, my_bars + stage * 8, policy);
+    }
+  };
+
+  // Many items, none of them long: a CTA takes one or several at a time, each with `team` of its warps from the first page to
+  // the finished rows; no record is handed over, and no team waits for another. It must not load the CTAs too unevenly: the
+  // fullest has `heaviest` pages, a share has total / grid and a fold per item that it meets.
+  // (Both measured, teams and shares: 41 sequences x 8 KV heads of 7-85 tokens 6.8 and 24.4 us; 64 x 8 of 300-500 tokens 22.3
+  // and 31.0; 80 x 2 with a window of 400 tokens 10.6 and 16.5; 64 x 2 of 1024-1280 tokens, a CTA each, 16.1 and 18.4.)
+  const int rounds = (items + gridDim.x - 1) / gridDim.x, heaviest = rounds * most_pages;
+  const int team = rounds <= 1 ? 8 : rounds <= 2 ? 4 : rounds <= 4 ? 2 : 1;
+  if (!chunked && most_pages <= kTeamPages * team &&
+      heaviest <= total / static_cast<int>(gridDim.x) + kSegmentPages * (2 + items / static_cast<int>(gridDim.x))) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (kScores) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (see below)
+    const int teams = kWarps / team, my_team = warp / team, member = warp - my_team * team;
+    auto team_meets = [&]() {
+      if (team == 1) __syncwarp(); else asm volatile("bar.sync %0, %1;" ::"r"(1 + my_team), "r"(32 * team) : "memory");
+    };
+    int used = 0, issued = 0;   // pages of this warp, through all its items
+#pragma unroll 1
+    for (int id = my_team * gridDim.x + cta; id < p.num_seqs * heads; id += teams * gridDim.x) {
+      const int seq = id / heads, head = id - seq * heads, entries = prefix[seq + 1] - prefix[seq];
+      if (entries == 0) continue;
+      const int n = entries > member ? (entries - member + team - 1) / team : 0;   // this warp's: member, member + team, ...
+      const int len = min(p.seq_lens[seq], p.max_blocks * kKvBlock), w0 = max(0, len - p.window), gap = skip[seq];
+      auto page_of = [&](int i) {
+        const int entry = member + team * i;
+        return entry >= p.sink_pages ? entry + gap : entry;
+      };
+      int tile = 0;
+      if (lane < n) tile = __ldg(p.tables + static_cast<int64_t>(seq) * p.max_blocks + page_of(lane)) * 2 * heads + head;
+      const int base = used;
+      auto request_up_to = [&](int end) {
+        for (; issued < end && !failed; ++issued) request(issued % kStages, __shfl_sync(0xffffffffu, tile, issued - base));
+      };
+      request_up_to(base + min(n, kStages));
+      uint32_t qb[8][2];
+      LoadQueries(p, seq, head, lane, qb);
+      float* scores = kScores ? p.scores + (static_cast<int64_t>(seq) * heads + head) * p.max_blocks * (kKvBlock * p.group) : nullptr;
+      Running run;
+      run.Clear();
+#pragma unroll 1
+      for (int i = 0; i < n && !failed; ++i) {
+        const int stage = used % kStages;
+        const bool arrived = MbarWait(my_bars + stage * 8, (used / kStages) & 1);
+        if (!__all_sync(0xffffffffu, arrived)) {
+          failed = true;
+          if (lane == 0) atomicExch(p.meta, 1);
+          break;
+        }
+        PageStep<kScores>(p, my_ring + stage * kStageBytes, off, qb, page_of(i) * kKvBlock, len, w0, scores, lane, run);
+        ++used;
+        __syncwarp();   // every lane is done with the stage before it is refilled
+        request_up_to(base + min(n, i + 1 + kStages));
+      }
+      LeaveInBuffer(run, obuf, mbuf, lbuf, warp, lane);
+      team_meets();
+      for (int q = member; q < p.group; q += team) {
+        float mx = -INFINITY, den = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int w = warp - member; w < warp - member + team; ++w) mx = fmaxf(mx, mbuf[q * kWarps + w]);
+        for (int w = warp - member; w < warp - member + team; ++w) {
+          const float f = Exp2(mbuf[q * kWarps + w] - mx);   // 0 for a warp that had no page
+          const float4 v = *reinterpret_cast<const float4*>(obuf + (w * kMaxGroup + q) * kHeadDim + ((4 * lane) ^ ((q >> 1) * 8)));
+          acc.x = fmaf(f, v.x, acc.x);
+          acc.y = fmaf(f, v.y, acc.y);
+          acc.z = fmaf(f, v.z, acc.z);
+          acc.w = fmaf(f, v.w, acc.w);
+          den = fmaf(f, lbuf[q * kWarps + w], den);
+        }
+        WriteRow<kScores>(p, seq, head * p.group + q, lane, acc, mx, den);
+      }
+      team_meets();
+    }
+    if (failed) {   // copies in flight get one more bounded chance to land before the shared memory goes away
+      for (int k = used; k < issued; ++k) MbarWait(my_bars + (k % kStages) * 8, (k / kStages) & 1);
+    }
+    return;
+  }
+
   int share_begin, share_end;
   int ctas, chunk_first = 0, chunk_last = 0;   // (chunked) the CTAs of this CTA's item
   if (chunked) {
@@ -253,11 +506,6 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   // ---- this warp's pages: share-relative indices warp, warp + 8, ...
   const int share_len = share_end - share_begin;
   const int n_mine = share_len > warp ? (share_len - warp + kWarps - 1) / kWarps : 0;
-  const uint32_t my_ring = SmemAddr(smem) + warp * (kStages * kStageBytes);
-  const uint32_t my_bars = SmemAddr(smem + kBarOff) + warp * (kStages * 8);
-  const uint64_t policy = L2PolicyEvictFirst();   // pages are read once per launch
-  bool failed = false;
-  int fail_at = 0;
 
   // Tile indices (4 KiB tiles of the pool; V lies `heads` tiles behind K) of 32 of this warp's pages at a time, one per
   // lane, read a batch ahead. A sequence's last page is marked: it holds the token that this step writes.
@@ -271,12 +519,6 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   };
   int tiles_cur = fetch_tiles(0);
   int tiles_next = n_mine > 32 ? fetch_tiles(1) : 0;
-  auto request = [&](int stage, int tile) {
-    if (lane == 0) {
-      MbarExpectTx(my_bars + stage * 8, kStageBytes);
-      TmaLoadPage(my_ring + stage * kStageBytes, &tile_map, tile & ~kNewestPageBit, my_bars + stage * 8, policy);
-    }
-  };
   // Under the overlap option this grid may run ahead of the previous kernel's end: pages that an earlier step wrote
   // are requested at once, a sequence's newest page - and everything else - after the wait.
   const int first = n_mine < kStages ? n_mine : kStages;
@@ -303,20 +545,6 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
       tiles_next = fetch_tiles((n_issue >> 5) + 1);
     }
   };
-  // ldmatrix offsets inside a stage: K rows as the A operand of S^T, V transposed as the A operand of O^T; dims 64..127
-  // of a tile sit one 2 KiB box further.
-  uint32_t koff[4], voff[4];
-  {
-    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_sel = lane >> 4;
-    const int v_row = (lane & 7) + (lane >> 4) * 8, v_sel = (lane >> 3) & 1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      koff[j] = k_row * 128 + (((2 * j + k_sel) ^ (k_row & 7)) << 4);
-      voff[j] = kPageBytes + v_row * 128 + (((2 * j + v_sel) ^ (v_row & 7)) << 4);
-    }
-  }
-  constexpr uint32_t kHiDims = 2048;
-
   // ---- one (sequence, KV head) segment of the share after the other
   int seg_begin = share_begin;
 #pragma unroll 1
@@ -329,16 +557,8 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
     const int gap = skip[sc.seq];
     const int seg_end_rel = seg_end - share_begin;
     const int entry0 = sc.entry - (seg_begin - share_begin);   // entry of the share's page `rel` is rel + entry0
-    uint32_t qb[8][2];   // B operand of S^T: query g of the group in column g, zeros past the group
-    {
-      const half* qrow = p.q + static_cast<int64_t>(sc.seq) * p.q_stride +
-                         (static_cast<int64_t>(sc.head) * p.group + g) * kHeadDim + 2 * tig;
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        qb[kk][0] = g < p.group ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * kk)) : 0u;
-        qb[kk][1] = g < p.group ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * kk + 8)) : 0u;
-      }
-    }
+    uint32_t qb[8][2];
+    LoadQueries(p, sc.seq, sc.head, lane, qb);
     const bool whole = seg_begin == item_begin && seg_end == item_end;
     int c_first = cta, c_last = cta;
     if (chunked) {
@@ -354,11 +574,8 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
     float* seg_scores = kScores ? p.scores + (static_cast<int64_t>(sc.seq) * heads + sc.head) * p.max_blocks * (kKvBlock * p.group) : nullptr;
     int seen = -1;   // thread 0: how many of the others had published when it looked
 
-    float o[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-
+    Running run;
+    run.Clear();
 #pragma unroll 1
     for (int rel = warp + kWarps * n_use; rel < seg_end_rel; rel += kWarps) {
       const int stage = n_use % kStages;
@@ -372,86 +589,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
       if (!failed) {
         const int entry = rel + entry0;
         const int page = entry >= p.sink_pages ? entry + gap : entry;
-        const int t0 = page * kKvBlock;
-        // token i of the page is visible if i < end and (i < sink or i >= win); all 16 are on a page in the middle
-        const int end = len - t0, sink = p.sinks - t0, win = w0 - t0;
-        const bool full = end >= kKvBlock && (sink >= kKvBlock || win <= 0);
-
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t a[4], a2[4];
-          Ldsm4(st + koff[j], a);
-          Ldsm4(st + koff[j] + kHiDims, a2);
-          Mma16816(s, a, qb[j][0], qb[j][1]);
-          Mma16816(s2, a2, qb[j + 4][0], qb[j + 4][1]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = (s[i] + s2[i]) * p.scale_log2e;
-        if (kScores) {   // [query][token]: the eight lanes of a query fill whole sectors
-          float* dst = seg_scores + static_cast<int64_t>(page) * (kKvBlock * p.group) + 2 * tig * kKvBlock + g;
-          if (2 * tig < p.group) {
-            __stcg(dst, s[0]);
-            __stcg(dst + 8, s[2]);
-          }
-          if (2 * tig + 1 < p.group) {
-            __stcg(dst + kKvBlock, s[1]);
-            __stcg(dst + kKvBlock + 8, s[3]);
-          }
-        }
-        auto visible = [&](int i) { return i < end && (i < sink || i >= win); };
-        if (!full) {
-          if (!visible(g)) s[0] = s[1] = -INFINITY;
-          if (!visible(g + 8)) s[2] = s[3] = -INFINITY;
-        }
-        float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
-        if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) {
-            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
-            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
-          }
-          const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-          const float a0 = Exp2(m0 - n0), a1 = Exp2(m1 - n1);
-          m0 = n0;
-          m1 = n1;
-          l0 *= a0;
-          l1 *= a1;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            o[i][0] *= a0;
-            o[i][1] *= a1;
-            o[i][2] *= a0;
-            o[i][3] *= a1;
-          }
-        }
-        const float p0 = Exp2(s[0] - m0), p1 = Exp2(s[1] - m1);
-        const float p2 = Exp2(s[2] - m0), p3 = Exp2(s[3] - m1);
-        l0 += p0 + p2;
-        l1 += p1 + p3;
-        const uint32_t b0 = MovmT(PackHalf2(p0, p1)), b1 = MovmT(PackHalf2(p2, p3));
-        if (full) {
-#pragma unroll
-          for (int mt = 0; mt < 8; ++mt) {
-            uint32_t a[4];
-            Ldsm4T(st + voff[mt & 3] + (mt >> 2) * kHiDims, a);
-            Mma16816(o[mt], a, b0, b1);
-          }
-        } else {
-          // V rows of invisible tokens may hold NaN, and 0 * NaN would poison the sums: cleared in registers.
-          const uint32_t k01 = (visible(2 * tig) ? 0x0000FFFFu : 0u) | (visible(2 * tig + 1) ? 0xFFFF0000u : 0u);
-          const uint32_t k23 = (visible(2 * tig + 8) ? 0x0000FFFFu : 0u) | (visible(2 * tig + 9) ? 0xFFFF0000u : 0u);
-#pragma unroll
-          for (int mt = 0; mt < 8; ++mt) {
-            uint32_t a[4];
-            Ldsm4T(st + voff[mt & 3] + (mt >> 2) * kHiDims, a);
-            a[0] &= k01;
-            a[1] &= k01;
-            a[2] &= k23;
-            a[3] &= k23;
-            Mma16816(o[mt], a, b0, b1);
-          }
-        }
+        PageStep<kScores>(p, st, off, qb, page * kKvBlock, len, w0, seg_scores, lane, run);
       }
       ++n_use;
       __syncwarp();   // every lane is done with the stage before it is refilled
@@ -463,28 +601,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
       if (may_read_inline && seen < 0) seen = LoadAcquire(ticket);   // warp 0 had fewer than two pages here
       others_done = may_read_inline && seen == others;
     }
-#pragma unroll
-    for (int off = 4; off < 32; off <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, off);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, off);
-    }
-    {
-      float* ob = obuf + (warp * kMaxGroup + 2 * tig) * kHeadDim;
-#pragma unroll
-      for (int mt = 0; mt < 8; ++mt) {   // columns permuted by the query pair: no bank is met twice
-        const int c0 = (16 * mt + g) ^ (tig * 8), c1 = (16 * mt + g + 8) ^ (tig * 8);
-        ob[c0] = o[mt][0];
-        ob[kHeadDim + c0] = o[mt][1];
-        ob[c1] = o[mt][2];
-        ob[kHeadDim + c1] = o[mt][3];
-      }
-      if (g == 0) {
-        mbuf[(2 * tig) * kWarps + warp] = m0;
-        mbuf[(2 * tig + 1) * kWarps + warp] = m1;
-        lbuf[(2 * tig) * kWarps + warp] = l0;
-        lbuf[(2 * tig + 1) * kWarps + warp] = l1;
-      }
-    }
+    LeaveInBuffer(run, obuf, mbuf, lbuf, warp, lane);
     __syncthreads();
     // From here on warp h has query head h of the group, lane i its columns 4i .. 4i + 3.
     const bool has_head = warp < p.group;
@@ -525,19 +642,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
                  lbuf[warp * kWarps + w], acc, den);
     }
     auto write_item = [&](const float4& a, float m, float l) {
-      if (!has_head) return;
-      const int qh = sc.head * p.group + warp;
-      half* dst = p.out + static_cast<int64_t>(sc.seq) * p.out_stride + static_cast<int64_t>(qh) * kHeadDim + d;
-      const half2 lo = __floats2half2_rn(a.x / l, a.y / l), hi = __floats2half2_rn(a.z / l, a.w / l);
-      if (p.wide_out) {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(AsU32(lo), AsU32(hi));
-      } else {
-        dst[0] = __low2half(lo);
-        dst[1] = __high2half(lo);
-        dst[2] = __low2half(hi);
-        dst[3] = __high2half(hi);
-      }
-      if (kScores && lane == 0) p.stats[static_cast<int64_t>(sc.seq) * heads * p.group + qh] = make_float2(m, 1.0f / l);
+      if (has_head) WriteRow<kScores>(p, sc.seq, sc.head * p.group + warp, lane, a, m, l);
     };
     // Few contributors: from registers, in CTA order with one common maximum, whoever does it.
     auto merge_few = [&]() {

@@ -182,6 +182,31 @@ def test_window_decode_batches(lens, window):
     assert torch.equal(first, out), "two launches gave different bits"
 
 
+@pytest.mark.parametrize("lens,q_heads,kv_heads,window,sinks", [
+    ([1 + 7 * i % 90 for i in range(41)], 64, 8, 10**6, 0), ([500 + i for i in range(64)], 24, 4, 30, 5),
+    ([512 - i % 16 for i in range(80)], 12, 2, 4096, 0),        # 32 pages each: a warp's share of items
+    ([513 + i % 3 for i in range(80)], 12, 2, 4096, 0),         # 33
+    ([0, 3, 0, 40] * 24, 16, 8, 33, 1), ([20] * 148, 1, 1, 9, 0), ([20] * 149, 1, 1, 9, 0), ([700] * 74, 6, 2, 16, 16)])
+def test_decode_many_small_items(lens, q_heads, kv_heads, window, sinks):
+    """More (sequence, KV head) items than CTAs, and the shapes around the border of the ways to cut them; window attention
+    and weights."""
+    c = Cache(lens, kv_heads, seed=len(lens))
+    q, out, qs, os_ = decode_case(c, q_heads, 0, 0, 0)
+    ws = K.window_attention_workspace(len(lens), c.mbps, q_heads, kv_heads, weights=True)
+    for _ in range(2):
+        K.launch_paged_window_attention_decode(out, os_, q, qs, c.pool, c.tables, c.seq_lens, len(lens), c.mbps, q_heads, kv_heads, D,
+                                               SCALE, window, sinks, ws)
+    check_decode(c, q, out, q_heads, window, sinks)
+    w = torch.zeros(c.blocks, kv_heads, PAGE, device="cuda")
+    out.fill_(7.0)
+    K.launch_paged_attention_decode_weights(out, os_, q, qs, c.pool, c.tables, c.seq_lens, len(lens), c.mbps, q_heads, kv_heads, D,
+                                            SCALE, w, ws)
+    check_decode(c, q, out, q_heads, 10**6, 0)
+    ref, tol = weights64(c, q, q_heads, torch.zeros_like(w))
+    assert bool(((w.double() - ref).abs() <= tol).all())
+    assert K.window_attention_health(ws) == 0
+
+
 def test_window_decode_lengths_beyond_the_table_are_cut_and_negative_ones_skipped():
     c = Cache([48, 48, 48], 2, seed=5, spare=0)
     c.seq_lens.copy_(torch.tensor([100000, -5, INT_MAX], dtype=torch.int32))
