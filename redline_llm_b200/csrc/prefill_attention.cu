@@ -45,6 +45,11 @@
 //    8 keys x 64 dims, 2 KiB between key groups, 1 KiB between the dim halves, one page per K = 16 slice -
 //    accumulated over all blocks in tensor-memory columns 256-383; read once at the end, divided by the row
 //    sum, rounded once.
+//  * With a sliding window and sinks (rl_launch_paged_window_prefill_attention) the same kernel, instantiated over a tile's
+//    LIST of visible pages (SpanOfTile below) instead of all pages up to the diagonal: rows mask by position in the blocks
+//    that hold an edge of the window, V rows that no row of the tile sees are cleared, everything else is as above. 2048 rows
+//    at context 8192 with a window of 1024: 35 us; 8192 rows with a window of 4096: 178 us, 880 TFLOP/s of visible pairs.
+//    Short windows are bound by a CTA's fixed 8 us and by 192 items on 148 SMs (ten blocks each), long ones by a block's softmax.
 // Every mbarrier wait is bounded and reports through rl_prefill_attention_health.
 #include <cuda.h>
 
@@ -815,16 +820,7 @@ EncodeTiledFn g_encode = nullptr;
 std::mutex g_mutex;
 int g_split_blocks = 0;   // 0: chosen per launch (ChooseSplitBlocks); > 0: forced (rl_prefill_attention_set_split_blocks)
 
-// Longest run of key blocks one CTA should take: a (tile, head) pair with more blocks is cut into equal runs.
-// The launch is replayed on the host the way the hardware runs it - CTAs start in grid order, each on the SM that
-// frees first - with costs measured on B200 (1.15 us per key block, 8 us of set-up and tear-down per CTA, kPublishUs
-// for a run's record, kCombineUs once for the kernel that combines the records), and the candidate with the shortest
-// makespan wins; on every chunk shape swept on B200 that choice was the best forced run length or level with it.
-// Cutting only the LONGEST tiles often does best (2048 rows at context 8192: runs of at most 60 blocks turn 192
-// items in two waves into 240 that level out, 120 -> 104 us); a prompt's last 128 rows against 32768 keys are cut
-// into a dozen runs each (263 -> 37 us). The choice depends on the chunk alone, so it is remembered across the
-// layers of a model.
-// Key blocks of query tile t; window = INT32_MAX and sinks = 0 for plain causal attention.
+// A chunk; window = INT32_MAX and sinks = 0 for plain causal attention.
 struct Chunk {
   int start, len, heads, window, sinks;
   int Tiles() const { return (len + kBM - 1) / kBM; }
@@ -838,6 +834,15 @@ struct Chunk {
   }
 };
 
+// Longest run of key blocks one CTA should take: a (tile, head) pair with more blocks is cut into equal runs.
+// The launch is replayed on the host the way the hardware runs it - CTAs start in grid order, each on the SM that
+// frees first - with costs measured on B200 (1.15 us per key block, 8 us of set-up and tear-down per CTA, kPublishUs
+// for a run's record, kCombineUs once for the kernel that combines the records), and the candidate with the shortest
+// makespan wins; on every chunk shape swept on B200 that choice was the best forced run length or level with it.
+// Cutting only the LONGEST tiles often does best (2048 rows at context 8192: runs of at most 60 blocks turn 192
+// items in two waves into 240 that level out, 120 -> 104 us); a prompt's last 128 rows against 32768 keys are cut
+// into a dozen runs each (263 -> 37 us). The choice depends on the chunk alone, so it is remembered across the
+// layers of a model.
 double SimulatedMakespan(const Chunk& chunk, int split_blocks, int sm_count, std::vector<double>& free_at) {
   constexpr double kBlockUs = 1.15, kSetupUs = 8.0, kPublishUs = 1.5, kCombineUs = 4.0;
   free_at.assign(sm_count, 0.0);                       // a min-heap of the times at which the SMs free up
