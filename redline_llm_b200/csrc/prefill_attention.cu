@@ -244,6 +244,11 @@ __device__ __forceinline__ uint32_t VisibleKeys(int base, int pos, int window, i
   return Below(pos + 1 - base) & (Below(sinks - base) | ~Below(pos - window + 1 - base));
 }
 
+template <bool kValue>
+struct Constant {
+  __device__ constexpr operator bool() const { return kValue; }
+};
+
 template <bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1)
 PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap q_map,
@@ -551,22 +556,33 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
       auto write_probabilities = [&](float ref) {
         const uint64_t scale2 = Pack2(p.scale_log2e, p.scale_log2e), neg_ref2 = Pack2(-ref, -ref);
         uint64_t sums = Pack2(0.0f, 0.0f);   // even keys, odd keys
+        auto sweep = [&](auto masked) {
 #pragma unroll
-        for (int c = 0; c < kScoreChunks; ++c) {
-          uint32_t packed[8];
+          for (int c = 0; c < kScoreChunks; ++c) {
+            uint32_t packed[8];
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float2 x = Unpack2(Fma2(Pack2(__uint_as_float(raw[c][i]), __uint_as_float(raw[c][i + 1])), scale2, neg_ref2));
-            float p0 = Ex2(x.x);
-            float p1 = Ex2(x.y);
-            if (diagonal) {
-              p0 = visible(c, i) ? p0 : 0.0f;
-              p1 = visible(c, i + 1) ? p1 : 0.0f;
+            for (int i = 0; i < 16; i += 2) {
+              const float2 x = Unpack2(Fma2(Pack2(__uint_as_float(raw[c][i]), __uint_as_float(raw[c][i + 1])), scale2, neg_ref2));
+              float p0 = Ex2(x.x);
+              float p1 = Ex2(x.y);
+              if (masked) {
+                p0 = visible(c, i) ? p0 : 0.0f;
+                p1 = visible(c, i + 1) ? p1 : 0.0f;
+              }
+              sums = Add2(sums, Pack2(p0, p1));
+              packed[i >> 1] = AsU32(__floats2half2_rn(p0, p1));
             }
-            sums = Add2(sums, Pack2(p0, p1));
-            packed[i >> 1] = AsU32(__floats2half2_rn(p0, p1));
+            TmemStore8(p_addr + 8 * c, packed);
           }
-          TmemStore8(p_addr + 8 * c, packed);
+        };
+        // Two copies of the sweep without a window, one with: each instance in the form that measured faster (2048 rows at
+        // context 8192: 100.4 and 104.1 us in two and one; 8192 rows with a window of 4096: 183.6 and 177.9).
+        if constexpr (kWindow) {
+          sweep(diagonal);
+        } else if (diagonal) {
+          sweep(Constant<true>());
+        } else {
+          sweep(Constant<false>());
         }
         const float2 sum01 = Unpack2(sums);
         return sum01.x + sum01.y;
