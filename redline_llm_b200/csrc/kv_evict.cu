@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1024 / kSelectThreads) SelectK
   __shared__ int local_bins[kBins];
   __shared__ int warp_sum[kSelectWarps], warp_equal[kSelectWarps];
   __shared__ uint32_t warp_lo[kSelectWarps], warp_hi[kSelectWarps], found_key;
-  __shared__ int found_bin, found_above, found_count;
+  __shared__ int found_bin, found_above, found_count, crowded;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int seq = blockIdx.x / cluster, rank = blockIdx.x % cluster, head = blockIdx.y;
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1024 / kSelectThreads) SelectK
       hi = max(hi, k);
     };
     clear_bins(sh.bins);
-    if (tid == 0) sh.listed = 0;
+    if (tid == 0) sh.listed = crowded = 0;
 #pragma unroll 1
     for (int q0 = q_first + tid; q0 < q_last; q0 += kLoadAhead * kSelectThreads) {
       int block[kLoadAhead];   // all table entries of a round in flight, then all weights
@@ -295,10 +295,8 @@ __global__ void __launch_bounds__(kSelectThreads, 1024 / kSelectThreads) SelectK
         continue;
       }
       if (found <= kRanked) {   // rank the last few against one another
-        if (tid == 0) found_count = 0;
-        __syncthreads();
         const bool in = tid < count && mine >= lo && mine <= hi;
-        if (in) crowd[atomicAdd(&found_count, 1)] = mine;
+        if (in) crowd[atomicAdd(&crowded, 1)] = mine;
         __syncthreads();
         if (in) {
           int larger = 0, equal = 0;
@@ -324,7 +322,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1024 / kSelectThreads) SelectK
   const int stretch = ((quads + kSelectThreads - 1) / kSelectThreads) * 32;
   const int q_begin = min(q_last, q_first + warp * stretch), q_end = min(q_last, q_begin + stretch);
   // of the four tokens from 4q on, one bit each: those that stay in any case, and those whose key equals the threshold
-  auto judge = [&](int q, uint32_t& sure, uint32_t& equal) {
+  auto classify = [&](int q, uint32_t& sure, uint32_t& equal) {
     sure = equal = 0;
     if (q >= q_end) return;
     const int t = 4 * q;
@@ -349,7 +347,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1024 / kSelectThreads) SelectK
 #pragma unroll 4
   for (int q0 = q_begin; q0 < q_end; q0 += 32) {
     uint32_t sure, equal;
-    judge(q0 + lane, sure, equal);
+    classify(q0 + lane, sure, equal);
     n_sure += __popc(sure);
     n_equal += __popc(equal);
   }
@@ -376,7 +374,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1024 / kSelectThreads) SelectK
 #pragma unroll 2
   for (int q0 = q_begin; q0 < q_end; q0 += 32) {
     uint32_t sure, equal;
-    judge(q0 + lane, sure, equal);
+    classify(q0 + lane, sure, equal);
     const uint32_t mine = __popc(sure) | __popc(equal) << 16;
     uint32_t incl = mine;
 #pragma unroll

@@ -379,7 +379,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   // each item in equal chunks with a CTA each. The longest chunk is longer than a share (74 pages against 62 where 24 items
   // of 380 meet 148 CTAs), but no CTA meets a second item, whose fold and hand-over cost it as much as kSegmentPages pages.
   // (Both measured, shares and chunks: 7 sequences of 3-2500 tokens, 28 items, 21.3 and 10.8 us; 8 x 4096, 16 items, 21.2
-  // and 14.4 us; 64 x 1024-1280, 128 items, stay with shares.)
+  // and 14.4 us.)
   int longest = 0;
   bool chunked = false;
   if (items <= static_cast<int>(gridDim.x)) {

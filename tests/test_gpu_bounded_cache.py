@@ -467,6 +467,31 @@ def test_evict_weights_that_share_a_bin(lens, kv, budget):
     check_evict(c, budget, 4, 100, some_weights(c, "crowded"), True)
 
 
+@pytest.mark.parametrize("rows,kv", [(96, 8), (10, 2)])
+def test_evict_rank_after_a_second_division(rows, kv):
+    """The limit lies among 500 neighbours that share a bin of the first division and are divided once more before the
+    last few are ranked: every warp must have read the count of its bin by then. Many items at once, again and again."""
+    n, budget = 2000, 1000
+    c = Cache([n] * rows, kv, seed=rows, spare=1)
+    band = 1.0 + torch.arange(500, device="cuda").double() * 2.0**-16   # apart by far more than an fp32 step
+    rest = torch.cat([torch.linspace(-1e4, -1e3, 750), torch.linspace(1e3, 1e4, 750)]).cuda().double()
+    values = torch.cat([band, rest]).float()
+    w = torch.zeros(c.blocks, kv, PAGE, device="cuda")
+    keep = torch.empty(rows, kv, budget, dtype=torch.int32, device="cuda")
+    for i, (b, s) in enumerate(c.slots):
+        for h in range(kv):
+            x = values[torch.randperm(n, generator=c.g, device="cuda")]
+            w[b, h, s] = x
+            keep[i, h] = torch.nonzero(x > x.sort().values[n - budget - 1]).flatten().int()
+    kept = torch.empty_like(keep)
+    new = torch.empty(rows, dtype=torch.int32, device="cuda")
+    for _ in range(20):
+        weights = w.clone()   # the selection reads these; what the pool holds does not matter here
+        kept.fill_(-9)
+        K.launch_kv_evict(c.pool, weights, c.tables, c.mbps, c.tables, c.mbps, c.seq_lens, new, kept, rows, kv, c.d, budget, 0, 0)
+        assert torch.equal(kept, keep)
+
+
 def test_evict_more_tokens_than_shared_memory_holds():
     """80 items, so one CTA each, two of them longer than the keys that a CTA keeps."""
     c = Cache([47001, 50] + [100] * 8, 8, seed=12)
