@@ -11,7 +11,7 @@
 //    crowd - one per thread - and are divided further until the last few are ranked against one another; then an ordered
 //    sweep writes the kept positions, each warp a stretch of the sequence, warp scans giving the ranks.
 //  * Move, 32 rows per warp: a lane looks up one row's source and destination, then the warp copies the rows 16 bytes a
-//    lane, eight rows in flight. In place a cluster of eight CTAs walks a (sequence, head) in cache order, every row of a round
+//    lane, eight rows in flight. In place a cluster of up to eight CTAs walks a (sequence, head) in cache order, every row of a round
 //    read before any of it is written: a row never moves to a higher slot, so what a round overwrites was read in it or
 //    before it.
 #include <mutex>
@@ -590,18 +590,25 @@ extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int
   const int rows = few ? kRowsInFlight : 32;
   const int64_t most = (longest + kMoveWarps * rows - 1) / (kMoveWarps * rows);
   const int64_t fair = (16LL * sms + items - 1) / items;
-  const int parts = in_place ? kCluster : static_cast<int>(most < fair ? most : fair);
-  // In place a cluster's round is all that its registers hold. While every item's cluster has SMs to itself, rounds of 2048
-  // rows, 256 of them in the registers of each CTA; where the items fill the machine several times over, small CTAs, four to
-  // an SM, whose rounds overlap (one sequence of 32768 tokens to 8192: 36.0 us wide, 46.9 small; 64 sequences to 2048 stay small: 52.6).
-  const bool wide = in_place && items * kCluster <= sms;
+  // In place a cluster's round is all that its registers hold. While every item's cluster of at least four CTAs has SMs to itself,
+  // 256 rows in the registers of each CTA, so up to 2048 a round; where the items fill the machine several times over, small CTAs, four
+  // to an SM, whose rounds overlap (one sequence of 32768 tokens to 8192: 36.0 us wide, 46.9 small; 5 x 4 items of 16000-32768 to 4099,
+  // clusters of four: 42.3 against 50.0; 64 sequences to 2048 stay small: 52.6). And no more CTAs than one round of the longest
+  // item fills (57 x 8 items to 12 tokens: 26.4 us, in clusters of eight 39.4).
+  int cluster_size = kCluster;
+  while (cluster_size > 4 && items * cluster_size > sms) cluster_size /= 2;
+  const bool wide = in_place && items * cluster_size <= sms;
+  if (!wide) cluster_size = kCluster;
+  const int64_t cta_rows = (wide ? kWideWarps : kMoveWarps) * (head_dim != 128 ? 1 : wide ? kWideRows : kRowsInFlight);
+  while (cluster_size > 1 && cta_rows * (cluster_size / 2) >= longest) cluster_size /= 2;
+  const int parts = in_place ? cluster_size : static_cast<int>(most < fair ? most : fair);
   auto kernel = head_dim == 128
                     ? (wide ? MoveKernel<true, 32, kWideRows, kWideWarps> : in_place ? MoveKernel<true, 32, kRowsInFlight, kMoveWarps>
                        : few ? MoveKernel<false, 32, kRowsInFlight, kMoveWarps> : MoveKernel<false, 32, 32, kMoveWarps>)
                     : (wide ? MoveKernel<true, 0, 0, kWideWarps> : in_place ? MoveKernel<true, 0, 0, kMoveWarps>
                        : few ? MoveKernel<false, 0, kRowsInFlight, kMoveWarps> : MoveKernel<false, 0, 32, kMoveWarps>);
   e = LaunchDependent(kernel, dim3(static_cast<unsigned>(num_seqs) * parts, num_kv_heads), dim3(wide ? kWideWarps * 32 : kMoveThreads), 0,
-                      in_place ? kCluster : 1, s, p, parts);
+                      in_place ? parts : 1, s, p, parts);
   if (e != cudaSuccess) return Fail(static_cast<int>(e), "%s (move): %s", fn, cudaGetErrorString(e));
   return LaunchStatus(fn);
 }

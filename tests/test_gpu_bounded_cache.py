@@ -492,6 +492,14 @@ def test_evict_rank_after_a_second_division(rows, kv):
         assert torch.equal(kept, keep)
 
 
+@pytest.mark.parametrize("rows,kv,budget,head_dim", [(n, kv, budget, d) for d in (D, 64) for n, kv in ((3, 2), (9, 4), (70, 2))
+                                                     for budget in (1, 8, 17, 64, 65, 130, 257, 513, 1025)])
+def test_evict_in_place_around_a_round(rows, kv, budget, head_dim):
+    """In place, clusters of one to eight CTAs: kept tokens at and next to what a CTA or a cluster has in registers."""
+    c = Cache([1100 + i % 7 for i in range(rows)], kv, seed=budget, head_dim=head_dim)
+    check_evict(c, budget, 0, 1, some_weights(c, "spread"), True, alias=True)
+
+
 def test_evict_more_tokens_than_shared_memory_holds():
     """80 items, so one CTA each, two of them longer than the keys that a CTA keeps."""
     c = Cache([47001, 50] + [100] * 8, 8, seed=12)
