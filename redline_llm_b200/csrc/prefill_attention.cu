@@ -496,7 +496,9 @@ PagedPrefillAttentionKernel(const Params p, const __grid_constant__ CUtensorMap 
     const int hw = warp >> 2;                        // which 64 keys of a block (and which 64 output dims at the end)
     const int my_pos = min(p.chunk_start + row0 + row, kv_len - 1);   // rows past the chunk are computed, never stored
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    float m_ref = -INFINITY, l = 0.0f;
+    // With a window a row's first blocks may show it nothing, or nothing but scores of -inf (keys that overflowed): against
+    // a finite reference those have weight zero.
+    float m_ref = kWindow ? -3.402823466e38f : -INFINITY, l = 0.0f;
     // This thread's 64 scores of a block are fetched from tensor memory once, all four loads in flight together,
     // and kept in registers for both passes. The fetch for block j+1 is made at the END of block j, before this
     // thread reports P_j: when all have reported P_j, both S buffers have been read out, and the MMA warp writes

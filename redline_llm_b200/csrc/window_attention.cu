@@ -160,13 +160,16 @@ __device__ __forceinline__ PageOffsets MakePageOffsets(int lane) {
   }
   return off;
 }
+// Where a running maximum starts: finite, so that a visible score of -inf (a key that overflowed) has weight zero on a page that
+// shows nothing else, and not the NaN of inf - inf.
+constexpr float kLowest = -3.402823466e38f;
 struct Running {
   float o[8][4];            // O^T: dims 16 i + g (+ 8) of queries 2 tig, 2 tig + 1
   float m0, m1, l0, l1;     // of the two queries; l is this lane's share of the sum
   __device__ __forceinline__ void Clear() {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    m0 = m1 = -INFINITY;
+    m0 = m1 = kLowest;
     l0 = l1 = 0.0f;
   }
 };

@@ -325,6 +325,61 @@ def test_window_prefill_scores_that_outgrow_the_reference():
     check_prefill(c, q, out, 1000, 400, 12, 600, 40, some=range(0, 400, 13))
 
 
+@pytest.mark.parametrize("window,sinks", [(20, 1), (1, 1), (40, 0), (5000, 0)])
+def test_a_visible_key_of_minus_infinity_has_weight_zero(window, sinks):
+    """The first and the newest token score -inf; each may be all that its page shows."""
+    lens = [17, 33, 300, 16, 2001, 4993]
+    c = Cache(lens, 2, seed=sinks + 3)
+    for i, n in enumerate(lens):
+        b, s = c.slots[i]
+        for t in (0, n - 1):
+            if (window, sinks) != (1, 1) or t > 0:   # one visible key has to be finite
+                c.pool[b[t], 0, :, s[t], 0] = float("-inf")
+    q, out, qs, os_ = decode_case(c, 12, 0, 0, 0)
+    q[:len(lens)].view(len(lens), 12, D)[:, :, 0] = 0.5
+    ws = K.window_attention_workspace(len(lens), c.mbps, 12, 2, weights=True)
+    w = torch.zeros(c.blocks, 2, PAGE, device="cuda")
+
+    def verify(window, sinks, weights):
+        for i, n in enumerate(lens):
+            t = torch.arange(n, device="cuda")
+            k, v = c.kv64(i)
+            seen = ((t < sinks) | (t >= n - window)) & torch.isfinite(k[0, :, 0])
+            ref, tol, p, ptol = attend64(q[i, :12 * D].double().view(2, -1, D), k, v, seen)
+            check(out[i].view(2, -1, D), ref, tol, f"sequence {i} of {n}")
+            if weights:
+                b, s = c.slots[i]
+                got = w[b, :, s].T.double()
+                want, room = torch.zeros_like(got), torch.zeros_like(got)
+                want[:, seen], room[:, seen] = p.sum(1), ptol.sum(1) + 9 * 2.0**-24 * p.sum(1)
+                assert bool(((got - want).abs() <= room).all())
+
+    K.launch_paged_attention_decode_weights(out, os_, q, qs, c.pool, c.tables, c.seq_lens, len(lens), c.mbps, 12, 2, D, SCALE, w, ws)
+    verify(5000, 0, True)
+    K.launch_paged_window_attention_decode(out, os_, q, qs, c.pool, c.tables, c.seq_lens, len(lens), c.mbps, 12, 2, D, SCALE, window,
+                                           sinks, ws)
+    verify(window, sinks, False)
+
+
+@pytest.mark.parametrize("start,rows,window,sinks", [(1000, 200, 100, 1), (0, 300, 50, 2), (6000, 64, 5000, 1)])
+def test_window_prefill_visible_keys_of_minus_infinity(start, rows, window, sinks):
+    """The sinks score -inf: for later rows of a tile they are all that the first block of keys shows."""
+    c = Cache([start + rows], 2, seed=rows)
+    b, s = c.slots[0]
+    first = sinks if start else sinks - 1   # from position 0 on, the first row sees nothing else
+    c.pool[b[sinks - first:sinks], 0, :, s[sinks - first:sinks], 0] = float("-inf")
+    q, out, qs, os_ = decode_case_rows(c, rows, 12, 1536, 1536)
+    q[:rows].view(rows, 12, D)[:, :, 0] = 0.5
+    run_prefill(c, q, out, qs, os_, start, rows, 12, window, sinks)
+    k, v = c.kv64(0)
+    t = torch.arange(start + rows, device="cuda")
+    for i in range(0, rows, 9):
+        p = start + i
+        seen = (t <= p) & ((t < sinks) | (t > p - window)) & torch.isfinite(k[0, :, 0])
+        ref, tol, _, _ = attend64(q[i, :12 * D].double().view(2, -1, D), k, v, seen)
+        check(out[i].view(2, -1, D), ref, tol, f"row {i}")
+
+
 def weights64(c, q, q_heads, old):
     """Expected weights and their tolerance after one step, from the old ones."""
     new, tol = old.double().clone(), torch.zeros_like(old, dtype=torch.float64)
