@@ -238,6 +238,12 @@ def _here(*tensors) -> None:
             raise KernelError(f"a tensor on {t.device} was given to a launch on cuda:{here}")
 
 
+def _holds(name: str, t, dtype: str, at_least: int) -> None:
+    """An array that a bounded-cache launcher writes: of another type, with gaps or shorter, it would be written past its end."""
+    if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or t.numel() < at_least:
+        raise KernelError(f"{name} must be a contiguous {dtype} tensor of at least {at_least} elements")
+
+
 def _workspace(bytes_needed: int, device):
     import torch
     return torch.zeros(max(16, bytes_needed), dtype=torch.uint8, device="cuda" if device is None else device)
@@ -283,6 +289,7 @@ def launch_paged_attention_decode_weights(out, out_row_stride, q, q_row_stride, 
     """Decode attention over the whole cache that adds each cached token's softmax probabilities, summed over the
     query heads of a group, to weights (float32 [num_blocks, num_kv_heads, 16], paged like the pool); the newest
     token's entry is set, not added to."""
+    _holds("weights", weights, "float32", 16 * num_kv_heads)
     _here(out, q, kv_pool_layer, block_tables, seq_lens, weights, workspace)
     _check(lib().rl_launch_paged_attention_decode_weights(
         _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_tables.data_ptr(),
@@ -320,6 +327,9 @@ def launch_kv_evict(kv_pool_layer, weights, block_tables, max_blocks_per_seq, ds
     """Shrinks each sequence's cache to `budget` tokens per KV head: the first `sinks`, the last `recent` and the
     heaviest of the rest, moved in cache order to the pages of dst_block_tables (the same tensor as block_tables: in
     place). kept (int32 [num_seqs, num_kv_heads, budget]) receives the slots they had, -1 behind the last."""
+    _holds("weights", weights, "float32", 16 * num_kv_heads)
+    _holds("new_seq_lens", new_seq_lens, "int32", num_seqs)
+    _holds("kept", kept, "int32", num_seqs * num_kv_heads * budget)
     _here(kv_pool_layer, weights, block_tables, dst_block_tables, seq_lens, new_seq_lens, kept)
     _check(lib().rl_launch_kv_evict(
         _ptr(kv_pool_layer), _ptr(weights), block_tables.data_ptr(), max_blocks_per_seq, dst_block_tables.data_ptr(),

@@ -114,3 +114,20 @@ def test_workspace_queries():
     assert L.rl_window_prefill_workspace_bytes(0, 1, 12, 1, 0, None) == NULL
     assert L.rl_window_attention_workspace_bytes(1, 1, 12, 2, 0, None) == NULL
     assert L.rl_window_attention_health(None, None) == NULL
+
+
+def test_arrays_that_would_be_written_past_their_end_are_refused():
+    """By the Python wrappers, before anything else is looked at."""
+    torch = pytest.importorskip("torch")
+    t = torch.zeros(4, 8, dtype=torch.int32)
+    lens, w, kept = torch.zeros(4, dtype=torch.int32), torch.zeros(9, 2, 16), torch.zeros(4, 2, 64, dtype=torch.int32)
+
+    def evict(w=w, new=lens, kept=kept):
+        K.launch_kv_evict(t, w, t, 8, t, 8, lens, new, kept, 4, 2, 128, 64, 4, 16)
+
+    for bad in (dict(w=w.half()), dict(w=w.double()), dict(w=torch.zeros(9, 2, 32)[:, :, ::2]), dict(kept=kept.short()),
+                dict(kept=kept[:3]), dict(kept=kept[:, :1].expand(4, 2, 64)), dict(new=lens.long()), dict(new=lens[:3])):
+        with pytest.raises(K.KernelError, match="must be a contiguous"):
+            evict(**bad)
+    with pytest.raises(K.KernelError, match="must be a contiguous"):
+        K.launch_paged_attention_decode_weights(t, 1536, t, 1536, t, t, lens, 4, 8, 12, 2, 128, 0.1, w.half(), t)
