@@ -251,12 +251,26 @@ _types = {}   # torch's type objects by name: comparing one is faster than spell
 
 
 def _holds(name: str, t, dtype: str, at_least: int) -> None:
-    """An array that a bounded-cache launcher writes: of another type, with gaps or shorter, it would be written past its end."""
+    """An array that a bounded-cache launcher writes, or takes addresses from: of another type, with gaps or shorter, the
+    launch would write past its end or into other pages."""
     if dtype not in _types:
         import torch
         _types[dtype] = getattr(torch, dtype)
     if t.dtype is not _types[dtype] or not t.is_contiguous() or t.numel() < at_least:
         raise KernelError(f"{name} must be a contiguous {dtype} tensor of at least {at_least} elements")
+
+
+def _rows_fit(t, rows: int, stride: int, width: int) -> None:
+    """The output rows of a bounded-cache attention launcher: 16-bit elements, the last row inside the tensor's memory."""
+    need = (rows - 1) * stride + width
+    if t.element_size() != 2 or (rows > 0 and t.numel() < need
+                                 and t.untyped_storage().nbytes() // 2 - t.storage_offset() < need):
+        raise KernelError(f"out must hold {rows} rows of {width} 16-bit elements at a stride of {stride}")
+
+
+def _weights_fit(weights, kv_pool_layer, head_dim: int) -> None:
+    """One weight per K row of the pool: the kernels find both by the same page numbers."""
+    _holds("weights", weights, "float32", kv_pool_layer.nbytes // (4 * head_dim) if head_dim > 0 else 1)
 
 
 def _workspace(bytes_needed: int, device):
@@ -291,6 +305,9 @@ def launch_paged_window_attention_decode(out, out_row_stride, q, q_row_stride, k
                                          window, sinks, workspace, stream=None, q_offset=0):
     """launch_paged_attention_decode over the first `sinks` and the last `window` cached tokens of each sequence;
     pages (and table entries) outside both are not read. 1 to 8 query heads per KV head."""
+    _holds("block_tables", block_tables, "int32", num_seqs * max_blocks_per_seq)
+    _holds("seq_lens", seq_lens, "int32", num_seqs)
+    _rows_fit(out, num_seqs, out_row_stride, num_q_heads * head_dim)
     _here(out, q, kv_pool_layer, block_tables, seq_lens, workspace)
     _check(lib().rl_launch_paged_window_attention_decode(
         _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_tables.data_ptr(),
@@ -304,7 +321,10 @@ def launch_paged_attention_decode_weights(out, out_row_stride, q, q_row_stride, 
     """Decode attention over the whole cache that adds each cached token's softmax probabilities, summed over the
     query heads of a group, to weights (float32 [num_blocks, num_kv_heads, 16], paged like the pool); the newest
     token's entry is set, not added to."""
-    _holds("weights", weights, "float32", 16 * num_kv_heads)
+    _weights_fit(weights, kv_pool_layer, head_dim)
+    _holds("block_tables", block_tables, "int32", num_seqs * max_blocks_per_seq)
+    _holds("seq_lens", seq_lens, "int32", num_seqs)
+    _rows_fit(out, num_seqs, out_row_stride, num_q_heads * head_dim)
     _here(out, q, kv_pool_layer, block_tables, seq_lens, weights, workspace)
     _check(lib().rl_launch_paged_attention_decode_weights(
         _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_tables.data_ptr(),
@@ -329,6 +349,8 @@ def launch_paged_window_prefill_attention(out, out_row_stride, q, q_row_stride, 
                                           head_dim, scale, window, sinks, workspace=None, stream=None, q_offset=0):
     """launch_paged_prefill_attention with a sliding window and sinks: row i sees the first `sinks` tokens and the
     last `window` up to its own position. Without a workspace no work is cut across CTAs (slower, same function)."""
+    _rows_fit(out, chunk_len, out_row_stride, num_q_heads * head_dim)
+    _holds("block_table_row", block_table_row, "int32", min(max_blocks_per_seq, (chunk_start + chunk_len + 15) // 16))
     _here(out, q, kv_pool_layer, block_table_row, workspace)
     _check(lib().rl_launch_paged_window_prefill_attention(
         _ptr(out), out_row_stride, _ptr(q, q_offset), q_row_stride, _ptr(kv_pool_layer), block_table_row.data_ptr(),
@@ -342,7 +364,10 @@ def launch_kv_evict(kv_pool_layer, weights, block_tables, max_blocks_per_seq, ds
     """Shrinks each sequence's cache to `budget` tokens per KV head: the first `sinks`, the last `recent` and the
     heaviest of the rest, moved in cache order to the pages of dst_block_tables (the same tensor as block_tables: in
     place). kept (int32 [num_seqs, num_kv_heads, budget]) receives the slots they had, -1 behind the last."""
-    _holds("weights", weights, "float32", 16 * num_kv_heads)
+    _weights_fit(weights, kv_pool_layer, head_dim)
+    _holds("block_tables", block_tables, "int32", num_seqs * max_blocks_per_seq)
+    _holds("dst_block_tables", dst_block_tables, "int32", num_seqs * dst_max_blocks_per_seq)
+    _holds("seq_lens", seq_lens, "int32", num_seqs)
     _holds("new_seq_lens", new_seq_lens, "int32", num_seqs)
     _holds("kept", kept, "int32", num_seqs * num_kv_heads * budget)
     _here(kv_pool_layer, weights, block_tables, dst_block_tables, seq_lens, new_seq_lens, kept)

@@ -131,3 +131,64 @@ def test_arrays_that_would_be_written_past_their_end_are_refused():
             evict(**bad)
     with pytest.raises(K.KernelError, match="must be a contiguous"):
         K.launch_paged_attention_decode_weights(t, 1536, t, 1536, t, t, lens, 4, 8, 12, 2, 128, 0.1, w.half(), t)
+
+
+def test_weights_must_cover_the_pool_and_tables_and_lengths_be_int32():
+    """The kernels address weights, tables and lengths by the pool's page numbers and the call's counts: an array with fewer
+    pages than the pool would be written past its end, 64-bit tables read as pairs of wrong page numbers. Refused by the
+    wrappers for every layout of the pool tensor, before a device is looked at."""
+    torch = pytest.importorskip("torch")
+    blocks, kv, d, rows, mb = 9, 2, 128, 4, 8
+    pool = torch.zeros(blocks, 2, kv, 16, d, dtype=torch.float16)
+    good = dict(w=torch.zeros(blocks, kv, 16), tab=torch.zeros(rows, mb, dtype=torch.int32),
+                dst=torch.zeros(rows, 4, dtype=torch.int32), lens=torch.zeros(rows, dtype=torch.int32),
+                out=torch.zeros(rows, 12 * d, dtype=torch.float16), pool=pool)
+    new, kept = torch.zeros(rows, dtype=torch.int32), torch.zeros(rows, kv, 64, dtype=torch.int32)
+    ws, q = torch.zeros(1 << 20, dtype=torch.uint8), torch.zeros(rows, 12 * d, dtype=torch.float16)
+
+    def evict(**kw):
+        a = dict(good, **kw)
+        K.launch_kv_evict(a["pool"], a["w"], a["tab"], mb, a["dst"], 4, a["lens"], new, kept, rows, kv, d, 64, 4, 16)
+
+    def weights(**kw):
+        a = dict(good, **kw)
+        K.launch_paged_attention_decode_weights(a["out"], 12 * d, q, 12 * d, a["pool"], a["tab"], a["lens"], rows, mb, 12, kv, d,
+                                                0.1, a["w"], ws)
+
+    def window(**kw):
+        a = dict(good, **kw)
+        K.launch_paged_window_attention_decode(a["out"], 12 * d, q, 12 * d, a["pool"], a["tab"], a["lens"], rows, mb, 12, kv, d,
+                                               0.1, 9, 0, ws)
+
+    def prefill(**kw):
+        a = dict(good, **kw)
+        K.launch_paged_window_prefill_attention(a["out"], 12 * d, q, 12 * d, a["pool"], a["tab"], mb, 60, 4, 12, kv, d, 0.1, 9, 0)
+
+    short = dict(w=good["w"][:-1])
+    for call in (evict, weights):
+        for bad in (short, dict(short, pool=pool.view(-1)), dict(w=good["w"][:1]), dict(w=good["w"].half())):
+            with pytest.raises(K.KernelError, match="weights must be"):
+                call(**bad)
+    for call in (evict, weights, window):
+        for bad in (dict(tab=good["tab"].long()), dict(tab=good["tab"][:3]), dict(tab=torch.zeros(rows, 2 * mb, dtype=torch.int32)[:, ::2])):
+            with pytest.raises(K.KernelError, match="block_tables must be"):
+                call(**bad)
+        for bad in (dict(lens=good["lens"].long()), dict(lens=good["lens"][:3])):
+            with pytest.raises(K.KernelError, match="seq_lens must be"):
+                call(**bad)
+    for bad in (dict(dst=good["dst"].long()), dict(dst=good["dst"][:3])):
+        with pytest.raises(K.KernelError, match="dst_block_tables must be"):
+            evict(**bad)
+    for bad in (dict(tab=good["tab"].long()), dict(tab=torch.zeros(3, dtype=torch.int32))):
+        with pytest.raises(K.KernelError, match="block_table_row must be"):
+            prefill(**bad)
+    for call in (weights, window, prefill):
+        for bad in (dict(out=good["out"].float()), dict(out=good["out"][:3].clone()), dict(out=torch.zeros(rows, 11 * d, dtype=torch.float16))):
+            with pytest.raises(K.KernelError, match="out must hold"):
+                call(**bad)
+    # rows inside wider ones are fine as long as the last one ends inside the memory
+    wide = torch.zeros(rows, 16 * d, dtype=torch.float16)
+    K._rows_fit(wide[:, :12 * d], rows, 16 * d, 12 * d)
+    K._rows_fit(wide[:, 4 * d:], rows, 16 * d, 12 * d)
+    with pytest.raises(K.KernelError, match="out must hold"):
+        K._rows_fit(wide[:, 5 * d:], rows, 16 * d, 12 * d)
