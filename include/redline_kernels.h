@@ -226,7 +226,8 @@ int rl_launch_decode_advance(int32_t* input_ids, int32_t* positions, int32_t* se
 int rl_attention_health(int* flag_out);
 
 /*
- * Test hook for the give-up path of the attention kernel's bounded waits, for launches made after the call:
+ * Test hook for the give-up path of the decode attention kernels' bounded waits - this one's and those of the two
+ * bounded-cache decode launchers, whose flag rl_window_attention_health reads - for launches made after the call:
  * with drop_first_copy != 0 one warp of the first CTA never requests its first K/V page and so waits for a
  * copy that cannot arrive; wait_cycles > 0 replaces the limit of every wait (about a second by default) so
  * that the test takes a millisecond. The kernel then raises the health flag, lets its other copies land,

@@ -36,6 +36,11 @@ int CurrentDeviceIndex();
 // attention kernel after its table walk), so they never read or write before the previous kernel of
 // the stream has completed; what overlaps is the launch itself and, for attention, the walk.
 extern bool g_launch_overlap;
+constexpr long long kWaitCycles = 2000000000LL;  // ~1 s: a load that never lands is reported, not waited for
+// rl_attention_test_wait_expiry: the limit of the decode attention kernels' bounded waits (kWaitCycles unless a test
+// shortened it), and whether the first CTA leaves its first copy out.
+extern long long g_wait_cycles;
+extern bool g_drop_first_copy;
 
 template <typename... KArgs, typename... Args>
 inline cudaError_t LaunchOverlapped(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,

@@ -109,7 +109,6 @@ constexpr int kMetaInts = kTicketOff + kMaxCtas;   // the item that starts in CT
 constexpr size_t kWorkspaceBytes =
     static_cast<size_t>(kMetaInts) * 4 + static_cast<size_t>(kMaxCtas) * 2 * kPartialFloats * 4;
 
-constexpr long long kWaitCycles = 2000000000LL;  // ~1 s: a load that never lands sets the error flag
 
 struct Params {
   half* out;
@@ -835,8 +834,6 @@ DeviceState g_state[kMaxDevices];
 EncodeTiledFn g_encode = nullptr;
 void* g_timeline = nullptr;  // diagnostics build only
 std::mutex g_mutex;
-long long g_wait_cycles = kWaitCycles;   // rl_attention_test_wait_expiry
-int g_drop_first_copy = 0;
 
 // First call per device: driver entry point, shared-memory opt-in, workspace.
 int EnsureReady(DeviceState** out_state) {
@@ -965,8 +962,8 @@ extern "C" int rl_attention_health(int* flag_out) {
 }
 
 extern "C" int rl_attention_test_wait_expiry(int drop_first_copy, int64_t wait_cycles) {
-  rl::attn::g_drop_first_copy = drop_first_copy != 0;
-  rl::attn::g_wait_cycles = wait_cycles > 0 ? wait_cycles : rl::attn::kWaitCycles;
+  rl::g_drop_first_copy = drop_first_copy != 0;
+  rl::g_wait_cycles = wait_cycles > 0 ? wait_cycles : rl::kWaitCycles;
   return RL_OK;
 }
 

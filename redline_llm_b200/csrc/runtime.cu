@@ -6,6 +6,8 @@
 
 namespace rl {
 bool g_launch_overlap = false;
+long long g_wait_cycles = kWaitCycles;
+bool g_drop_first_copy = false;
 namespace {
 thread_local char g_error[512] = "";
 constexpr int kMaxDevices = 64;

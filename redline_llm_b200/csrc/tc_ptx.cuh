@@ -11,8 +11,6 @@
 namespace rl {
 namespace tc {
 
-constexpr long long kWaitCycles = 2000000000LL;  // ~1 s: a wait that never completes is reported, not spun on
-
 
 __device__ __forceinline__ uint32_t SmemAddr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -34,12 +32,13 @@ __device__ __forceinline__ bool MbarTryWait(uint32_t bar, int parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait: false when the phase never completed within kWaitCycles.
-__device__ __forceinline__ bool MbarWait(uint32_t bar, int parity) {
+// Bounded wait: false when the phase never completed within `limit` cycles. Lanes of a warp may come back with different
+// answers: vote before anything that needs the whole warp.
+__device__ __forceinline__ bool MbarWait(uint32_t bar, int parity, long long limit = kWaitCycles) {
   if (MbarTryWait(bar, parity)) return true;
   const long long t0 = clock64();
   while (!MbarTryWait(bar, parity)) {
-    if (clock64() - t0 > kWaitCycles) return false;
+    if (clock64() - t0 > limit) return false;
   }
   return true;
 }

@@ -98,6 +98,8 @@ struct Params {
   float* weights;
   bool wide_out;       // out rows are 8-byte aligned
   bool run_ahead;      // the overlap option: lengths, tables and all but the newest pages may be read before the wait
+  bool drop_first_copy;   // test hook: warp 0 of CTA 0 never requests its first page, so its wait must run out
+  long long wait_cycles;  // limit of every mbarrier wait
 };
 
 // A page's K tile and V tile of one KV head, 8 KiB, in one copy into this CTA's shared memory (no multicast).
@@ -397,8 +399,9 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   const PageOffsets off = MakePageOffsets(lane);
   bool failed = false;
   int fail_at = 0;
-  auto request = [&](int stage, int tile) {
-    if (lane == 0) {
+  auto request = [&](int k, int tile) {   // this warp's k-th page
+    const int stage = k % kStages;
+    if (lane == 0 && !(p.drop_first_copy && k == 0 && blockIdx.x == 0 && warp == 0)) {
       MbarExpectTx(my_bars + stage * 8, kStageBytes);
       TmaLoadPage(my_ring + stage * kStageBytes, &tile_map, tile & ~kNewestPageBit, my_bars + stage * 8, policy);
     }
@@ -434,7 +437,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
       if (lane < n) tile = __ldg(p.tables + static_cast<int64_t>(seq) * p.max_blocks + page_of(lane)) * 2 * heads + head;
       const int base = used;
       auto request_up_to = [&](int end) {
-        for (; issued < end && !failed; ++issued) request(issued % kStages, __shfl_sync(0xffffffffu, tile, issued - base));
+        for (; issued < end && !failed; ++issued) request(issued, __shfl_sync(0xffffffffu, tile, issued - base));
       };
       request_up_to(base + min(n, kStages));
       uint32_t qb[8][2];
@@ -445,7 +448,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
 #pragma unroll 1
       for (int i = 0; i < n && !failed; ++i) {
         const int stage = used % kStages;
-        const bool arrived = MbarWait(my_bars + stage * 8, (used / kStages) & 1);
+        const bool arrived = MbarWait(my_bars + stage * 8, (used / kStages) & 1, p.wait_cycles);
         if (!__all_sync(0xffffffffu, arrived)) {
           failed = true;
           if (lane == 0) atomicExch(p.meta, 1);
@@ -476,7 +479,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
       team_meets();
     }
     if (failed) {   // copies in flight get one more bounded chance to land before the shared memory goes away
-      for (int k = used; k < issued; ++k) MbarWait(my_bars + (k % kStages) * 8, (k / kStages) & 1);
+      for (int k = used; k < issued; ++k) MbarWait(my_bars + (k % kStages) * 8, (k / kStages) & 1, p.wait_cycles);
     }
     return;
   }
@@ -541,7 +544,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
   }
   int n_issue = first, n_use = 0;
   auto issue_one = [&]() {
-    request(n_issue % kStages, __shfl_sync(0xffffffffu, tiles_cur, n_issue & 31));
+    request(n_issue, __shfl_sync(0xffffffffu, tiles_cur, n_issue & 31));
     ++n_issue;
     if ((n_issue & 31) == 0) {
       tiles_cur = tiles_next;
@@ -583,10 +586,13 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
     for (int rel = warp + kWarps * n_use; rel < seg_end_rel; rel += kWarps) {
       const int stage = n_use % kStages;
       const uint32_t st = my_ring + stage * kStageBytes;
-      if (!failed && !MbarWait(my_bars + stage * 8, (n_use / kStages) & 1)) {
-        failed = true;
-        fail_at = n_use;
-        if (lane == 0) atomicExch(p.meta, 1);
+      if (!failed) {   // (the whole warp goes on or none of it: a page's products and shuffles need all lanes)
+        const bool arrived = MbarWait(my_bars + stage * 8, (n_use / kStages) & 1, p.wait_cycles);
+        if (!__all_sync(0xffffffffu, arrived)) {
+          failed = true;
+          fail_at = n_use;
+          if (lane == 0) atomicExch(p.meta, 1);
+        }
       }
       if (may_read_inline && tid == 0 && seen < 0 && rel + 2 * kWarps >= seg_end_rel) seen = LoadAcquire(ticket);
       if (!failed) {
@@ -733,7 +739,7 @@ DecodeKernel(const Params p, const __grid_constant__ CUtensorMap tile_map) {
     seg_begin = seg_end;
   }
   if (failed) {   // copies in flight get one more bounded chance to land before the shared memory goes away
-    for (int k = fail_at; k < n_issue; ++k) MbarWait(my_bars + (k % kStages) * 8, (k / kStages) & 1);
+    for (int k = fail_at; k < n_issue; ++k) MbarWait(my_bars + (k % kStages) * 8, (k / kStages) & 1, p.wait_cycles);
   }
 }
 
@@ -923,6 +929,8 @@ int Launch(const Call& c) {
   float2* stats = reinterpret_cast<float2*>(ws + kMetaBytes + kRecordBytes);
   float* scores = reinterpret_cast<float*>(ws + kMetaBytes + kRecordBytes + StatsBytes(c.num_seqs, c.q_heads));
   p.run_ahead = g_launch_overlap;
+  p.drop_first_copy = g_drop_first_copy;
+  p.wait_cycles = g_wait_cycles;
   p.wide_out = (reinterpret_cast<uintptr_t>(c.out) & 7) == 0 && (c.out_row_stride & 3) == 0;
   const int64_t pages = LongestList(c);   // no more CTAs than shares of kMinPagesPerCta pages can exist
   const int sms = CurrentDeviceFacts().sm_count < kMaxCtas ? CurrentDeviceFacts().sm_count : kMaxCtas;

@@ -672,6 +672,38 @@ def test_decode_output_rows_of_any_alignment(shift, stride):
     assert bool((buf[:shift] == 7.0).all()) and bool((buf[shift + 3 * stride:] == 7.0).all())
 
 
+@pytest.mark.parametrize("lens", [[700, 33, 1500], [900 + i for i in range(70)] + [8000] * 3, [5 + i for i in range(90)]],
+                         ids=["chunks", "shares", "teams"])
+def test_a_wait_that_runs_out_is_reported_and_the_next_launch_is_right(lens):
+    """The give-up path of the decode kernels' bounded waits, for each way to deal the pages: through the test hook one
+    warp never requests its first page, so its wait (shortened to about a millisecond) runs out. The launch comes back,
+    rl_window_attention_health says so once, and the next ordinary launch on the same workspace is correct."""
+    c = Cache(lens, 2, seed=len(lens))
+    rows = len(lens)
+    q, out, qs, os_ = decode_case(c, 12, 0, 0, 0)
+    ws = K.window_attention_workspace(rows, c.mbps, 12, 2, weights=True)
+    w = torch.zeros(c.blocks, 2, PAGE, device="cuda")
+
+    def window():
+        K.launch_paged_window_attention_decode(out, os_, q, qs, c.pool, c.tables, c.seq_lens, rows, c.mbps, 12, 2, D, SCALE, 10**6, 0, ws)
+
+    def weights():
+        K.launch_paged_attention_decode_weights(out, os_, q, qs, c.pool, c.tables, c.seq_lens, rows, c.mbps, 12, 2, D, SCALE, w, ws)
+
+    for launch in (window, weights):
+        try:
+            K.attention_test_wait_expiry(True, 2_000_000)
+            launch()
+            assert K.window_attention_health(ws) == 1, "the wait that ran out was not reported"
+            assert K.window_attention_health(ws) == 0, "the flag is cleared by the query that reported it"
+        finally:
+            K.attention_test_wait_expiry(False, 0)
+        out.fill_(7.0)
+        launch()
+        check_decode(c, q, out, 12, 10**6, 0)
+        assert K.window_attention_health(ws) == 0
+
+
 def test_tensors_elsewhere_are_refused():
     c = Cache([40], 2, seed=71)
     q, out, qs, os_ = decode_case(c, 12, 0, 0, 0)
