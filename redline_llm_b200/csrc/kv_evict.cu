@@ -37,7 +37,6 @@ struct Params {
   int sinks;
   int recent;
   int cached_keys;   // keys that fit the select kernel's shared memory
-  bool hold;         // the overlap option is on: nothing behind the move starts before its writes are done
 };
 
 // Weights as unsigned integers that compare the same way: 0 for a NaN, -0 like +0.
@@ -409,7 +408,6 @@ constexpr int kCluster = 8;
 // kLookup: rows a warp looks up at a time; in place (the K = 128 form) also the rows it has in registers at a time.
 template <bool kInPlace, int kRowWords, int kLookup, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, kWarps > kMoveWarps ? 1 : 4) MoveKernel(const Params p, int parts) {
-  if (!p.hold) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int seq = blockIdx.x / parts, part = blockIdx.x % parts, head = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -494,10 +492,11 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps > kMoveWarps ? 1 : 4) Move
     }
     if (moves) p.weights[weight_to] = weight;
   }
-  // Under the overlap option a decode launch behind this one requests pages and reads lengths before its own wait. It is
-  // then not released early, starts when every block here has ended, and by then these writes are done. (Two of 57 us for
-  // 64 sequences to 2048 tokens.)
-  if (p.hold) __threadfence();
+  // Under the overlap option a decode launch behind this one requests pages and reads lengths before its own wait. So
+  // dependents are not released early: they start when every block here has ended, and by then these writes are done. The
+  // option is the launching host's state when it comes to the DECODE launch, which this one cannot know: it always holds.
+  // (Released at the start it would take 54.9 us in place of 57.0 for 64 sequences to 2048 tokens.)
+  __threadfence();
 }
 
 // First use on a device: the selection's shared memory.
@@ -563,7 +562,6 @@ extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int
   p.sinks = sinks;
   p.recent = recent;
   const int64_t items = static_cast<int64_t>(num_seqs) * num_kv_heads;
-  p.hold = g_launch_overlap;
   p.cached_keys = static_cast<int>(tokens < kMaxCachedKeys ? tokens : kMaxCachedKeys);
   const int rc = EnsureReady(fn);
   if (rc != RL_OK) return rc;

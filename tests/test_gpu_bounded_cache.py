@@ -818,6 +818,35 @@ def test_with_dependent_launch_on_a_step_sees_what_the_launches_before_it_wrote(
                 assert torch.equal(a.nan_to_num(7.0) if a.is_floating_point() else a, b.nan_to_num(7.0) if b.is_floating_point() else b)
 
 
+@pytest.mark.parametrize("in_place", [True, False])
+def test_the_overlap_option_may_change_between_an_eviction_and_the_decode_behind_it(in_place):
+    """Launched with the option off, and the decode behind it with the option on: it reads lengths and older pages ahead of
+    its wait, and has to see the moved ones."""
+    rows, kv, heads, budget = 40, 2, 12, 1024
+    outs = []
+    for overlap in (False, True):
+        got = []
+        for run in range(8):
+            c = Cache([3000 + 7 * i for i in range(rows)], kv, seed=90, extra_pages=rows * budget // PAGE)
+            w = some_weights(c, "spread")
+            dst = c.tables if in_place else c.free[:rows * budget // PAGE].view(rows, -1).int().contiguous()
+            mb = dst.shape[1]
+            q, out, qs, os_ = decode_case(c, heads, 0, 0, 0)
+            kept = torch.zeros(rows, kv, budget, dtype=torch.int32, device="cuda")
+            ws = K.window_attention_workspace(rows, c.mbps, heads, kv)
+            torch.cuda.synchronize()
+            K.launch_kv_evict(c.pool, w, c.tables, c.mbps, dst, mb, c.seq_lens, c.seq_lens, kept, rows, kv, D, budget, 4, 100)
+            K.set_attention_prologue_overlap(overlap)
+            try:
+                K.launch_paged_window_attention_decode(out, os_, q, qs, c.pool, dst, c.seq_lens, rows, mb, heads, kv, D, SCALE, 10**6, 0, ws)
+            finally:
+                K.set_attention_prologue_overlap(False)
+            got.append(out.clone())
+        outs.append(got)
+    for x in outs[0] + outs[1]:
+        assert torch.equal(x, outs[0][0])
+
+
 def test_a_request_with_a_bounded_cache():
     """The operators as a serving loop uses them, against a 64-bit model of the same loop: a prompt ingested in two
     chunks with window attention, decode steps that scatter one token and accumulate weights, an eviction in place
