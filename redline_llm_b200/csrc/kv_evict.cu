@@ -495,7 +495,10 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps > kMoveWarps ? 1 : 4) Move
   // Under the overlap option a decode launch behind this one requests pages and reads lengths before its own wait. So
   // dependents are not released early: they start when every block here has ended, and by then these writes are done. The
   // option is the launching host's state when it comes to the DECODE launch, which this one cannot know: it always holds.
-  // (Released at the start it would take 54.9 us in place of 57.0 for 64 sequences to 2048 tokens.)
+  // (Released at the start it would take 54.9 us in place of 57.0 for 64 sequences to 2048 tokens.) Those pages are
+  // fetched by tensor copies, which go by the asynchronous proxy: the first fence orders the rows for them, on the side
+  // that wrote them. (Once more ahead of the decode kernels' early copies it would cost each of their launches 0.3 us.)
+  asm volatile("fence.proxy.async;" ::: "memory");
   __threadfence();
 }
 

@@ -847,6 +847,56 @@ def test_the_overlap_option_may_change_between_an_eviction_and_the_decode_behind
         assert torch.equal(x, outs[0][0])
 
 
+@pytest.mark.parametrize("in_place", [True, False])
+def test_both_decode_kernels_read_moved_pages_early(in_place):
+    """With the overlap option on, decode launches right behind an eviction request the moved rows by tensor copies ahead of
+    their wait: the same bits as with the option off, for the full and the window kernel, through graph replays."""
+    rows, kv, heads, budget = 24, 2, 12, 512
+    c = Cache([1200 + 31 * i for i in range(rows)], kv, seed=91, extra_pages=rows * budget // PAGE)
+    w = some_weights(c, "spread")
+    dst = c.tables if in_place else c.free[:rows * budget // PAGE].view(rows, -1).int().contiguous()
+    mb = dst.shape[1]
+    q, full, qs, os_ = decode_case(c, heads, 0, 0, 0)
+    window = full.clone()
+    new = torch.zeros_like(c.seq_lens)
+    kept = torch.zeros(rows, kv, budget, dtype=torch.int32, device="cuda")
+    ws = K.window_attention_workspace(rows, c.mbps, heads, kv)
+    lens0, pool0, w0 = c.seq_lens.clone(), c.pool.clone(), w.clone()
+
+    def go(first, second):
+        K.launch_kv_evict(c.pool, w, c.tables, c.mbps, dst, mb, c.seq_lens, new, kept, rows, kv, D, budget, 4, 100)
+        for name in (first, second):
+            if name == "full":
+                K.launch_paged_attention_decode(full, os_, q, qs, c.pool, dst, new, rows, mb, heads, kv, D, SCALE)
+            else:
+                K.launch_paged_window_attention_decode(window, os_, q, qs, c.pool, dst, new, rows, mb, heads, kv, D, SCALE, 300, 4, ws)
+
+    results = []
+    for overlap in (False, True):
+        K.set_attention_prologue_overlap(overlap)
+        try:
+            for order in (("full", "window"), ("window", "full")):
+                g = torch.cuda.CUDAGraph()
+                go(*order)
+                torch.cuda.synchronize()
+                with torch.cuda.graph(g):
+                    go(*order)
+                for _ in range(6):
+                    c.pool.view(torch.int16).copy_(pool0.view(torch.int16))
+                    w.copy_(w0)
+                    new.zero_()
+                    full.fill_(7.0), window.fill_(7.0)
+                    torch.cuda.synchronize()
+                    g.replay()
+                    torch.cuda.synchronize()
+                    results.append((full.clone(), window.clone()))
+        finally:
+            K.set_attention_prologue_overlap(False)
+    assert torch.equal(c.seq_lens, lens0)
+    for a, b in results:
+        assert torch.isfinite(a[:rows]).all() and torch.equal(a, results[0][0]) and torch.equal(b, results[0][1])
+
+
 def test_a_request_with_a_bounded_cache():
     """The operators as a serving loop uses them, against a 64-bit model of the same loop: a prompt ingested in two
     chunks with window attention, decode steps that scatter one token and accumulate weights, an eviction in place
