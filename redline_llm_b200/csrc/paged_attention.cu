@@ -448,11 +448,9 @@ PagedAttentionSplitKernel(const Params p, const __grid_constant__ CUtensorMap ti
     for (int rel = warp + kWarps * n_use; rel < seg_end_rel; rel += kWarps) {
       const int stage = n_use % kStages;
       const uint32_t st = my_ring + stage * kStageBytes;
-      if (!failed && !MbarWait(my_bars + stage * 8, (n_use / kStages) & 1, p.wait_cycles)) {
-        failed = true;
-        fail_at = n_use;
-        if (lane == 0) atomicExch(p.meta, 1);
-      }
+      // A wait may run out on some lanes only, and a page's products and shuffles need them all: the vote on the maximum
+      // below carries this one too (a vote of its own costs 0.3 % of 64 x 8192-32768 tokens). Until then the page is garbage.
+      const bool lost = !failed && !MbarWait(my_bars + stage * 8, (n_use / kStages) & 1, p.wait_cycles);
       if (n_use == 0) { RL_STAMP(2); }
       if (may_read_inline && tid == 0 && seen < 0 && rel + 2 * kWarps >= seg_end_rel)
         asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(p.meta + kTicketOff + c_first) : "memory");
@@ -475,7 +473,12 @@ PagedAttentionSplitKernel(const Params p, const __grid_constant__ CUtensorMap ti
         s[2] = g + 8 < valid ? (s[2] + s2[2]) * p.scale_log2e : -INFINITY;
         s[3] = g + 8 < valid ? (s[3] + s2[3]) * p.scale_log2e : -INFINITY;
         float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
-        if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
+        if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1 || lost)) {
+          if (__any_sync(0xffffffffu, lost)) {   // given up: no later page is waited for or requested
+            failed = true;
+            fail_at = n_use;
+            if (lane == 0) atomicExch(p.meta, 1);
+          }
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) {
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
