@@ -297,7 +297,10 @@ PagedAttentionSplitKernel(const Params p, const __grid_constant__ CUtensorMap ti
     __syncthreads();
   }
   const long long total = static_cast<long long>(heads) * prefix[num_seqs];
-  if (total == 0) return;
+  if (total == 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // this grid never completes ahead of the one before it
+    return;
+  }
   const long long share_begin = ShareBegin(blockIdx.x, total, gridDim.x);
   const long long share_end = ShareBegin(blockIdx.x + 1, total, gridDim.x);
   if (share_begin >= share_end) return;

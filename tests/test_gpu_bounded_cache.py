@@ -897,6 +897,45 @@ def test_both_decode_kernels_read_moved_pages_early(in_place):
         assert torch.isfinite(a[:rows]).all() and torch.equal(a, results[0][0]) and torch.equal(b, results[0][1])
 
 
+@pytest.mark.parametrize("kernel", ["full", "window", "weights"])
+def test_a_decode_launch_without_any_token_keeps_the_order_of_its_neighbours(kernel):
+    """With the overlap option on: a long kernel that releases its dependents early, a decode launch whose sequences are all
+    empty, and a kernel that reads what the first one wrote."""
+    c = Cache([0, 0, 0], 2, seed=92)
+    q, out, qs, os_ = decode_case(c, 12, 0, 0, 0)
+    ws = K.window_attention_workspace(3, c.mbps, 12, 2, weights=True)
+    w = torch.zeros(c.blocks, 2, PAGE, device="cuda")
+    rows, hidden = 100000, 1536
+    x = torch.randn(rows, hidden, generator=c.g, device="cuda").half()
+    gain = torch.ones(hidden, dtype=torch.float16, device="cuda")
+    mid, last = torch.zeros_like(x), torch.zeros_like(x)
+
+    def go():
+        K.launch_rms_norm(mid, x, gain, rows, hidden, 1e-6)
+        if kernel == "full":
+            K.launch_paged_attention_decode(out, os_, q, qs, c.pool, c.tables, c.seq_lens, 3, c.mbps, 12, 2, D, SCALE)
+        elif kernel == "window":
+            K.launch_paged_window_attention_decode(out, os_, q, qs, c.pool, c.tables, c.seq_lens, 3, c.mbps, 12, 2, D, SCALE, 9, 0, ws)
+        else:
+            K.launch_paged_attention_decode_weights(out, os_, q, qs, c.pool, c.tables, c.seq_lens, 3, c.mbps, 12, 2, D, SCALE, w, ws)
+        K.launch_rms_norm(last, mid, gain, rows, hidden, 1e-6)
+
+    go()
+    torch.cuda.synchronize()
+    want = last.clone()
+    K.set_attention_prologue_overlap(True)
+    try:
+        for _ in range(5):
+            mid.zero_(), last.zero_()
+            torch.cuda.synchronize()
+            go()
+            torch.cuda.synchronize()
+            assert torch.equal(last, want)
+    finally:
+        K.set_attention_prologue_overlap(False)
+    assert bool((out == 7.0).all())
+
+
 def test_a_request_with_a_bounded_cache():
     """The operators as a serving loop uses them, against a 64-bit model of the same loop: a prompt ingested in two
     chunks with window attention, decode steps that scatter one token and accumulate weights, an eviction in place
