@@ -156,6 +156,7 @@ class Request:
     total_blocks: int = 0       # pages its longest cache would fill
     need: int = 0               # pages it may hold at a time, reserved at admission
     trimmed: int = 0            # pages from here on have not been looked at by trim()
+    given_back: int = 0         # entries of `blocks` that trim() made the padding block
 
     @property
     def seq_len(self) -> int:   # tokens the next decode step attends to, including the new one
@@ -215,8 +216,9 @@ class Scheduler:
             if r.blocks[k] != DUMMY_BLOCK:
                 self.alloc.free_block(r.blocks[k])
                 r.blocks[k] = DUMMY_BLOCK
+                r.given_back += 1
         r.trimmed = max(r.trimmed, last)
-        live = sum(1 for b in r.blocks if b != DUMMY_BLOCK)
+        live = len(r.blocks) - r.given_back   # counted along: walking the list after every step would grow with the context
         more = min(r.need - live, r.total_blocks - len(r.blocks)) - r.reserved_left
         if more > 0:
             self.alloc.reserve(more)
@@ -267,6 +269,7 @@ class Scheduler:
             if b != DUMMY_BLOCK:
                 self.alloc.free_block(b)
         r.blocks = []
+        r.given_back = 0
         self.alloc.unreserve(r.reserved_left)
         r.reserved_left = 0
         if r in self.running:

@@ -83,3 +83,38 @@ def test_without_a_window_nothing_is_trimmed():
     before = list(r.blocks)
     s.trim(r, 1000)
     assert r.blocks == before and s.held_blocks() > 1 << 20
+
+
+def test_the_host_work_of_a_decode_step_does_not_grow_with_the_context():
+    """trim() runs after every decode step of every request: over a whole request it looks at each page a fixed number of
+    times, however long the list of pages has become."""
+    class Counted(list):
+        looks = 0
+
+        def __iter__(self):
+            for x in list.__iter__(self):
+                Counted.looks += 1
+                yield x
+
+        def __getitem__(self, k):
+            Counted.looks += 1
+            return list.__getitem__(self, k)
+
+    a = BlockAllocator(60)
+    s = Scheduler(a, 1, 1 << 20, 32, window=64, sinks=20)
+    r = Request(0, [1] * 32, 8000, ignore_eos=True)
+    s.enqueue(r)
+    s.plan_step()
+    r.blocks = Counted(r.blocks)
+    r.prefilled = r.cached = 32
+    s.trim(r, 32)
+    for _ in range(6000):
+        assert s.plan_step()[0] == "decode"
+        r.cached += 1
+        s.trim(r, r.cached)
+        held = [b for b in list.__iter__(r.blocks) if b != DUMMY_BLOCK]
+        assert len(held) <= s.held_blocks()
+        assert r.reserved_left + len(held) <= r.need
+    assert Counted.looks <= 4 * len(r.blocks), f"{Counted.looks} looks at {len(r.blocks)} pages"
+    s.release(r)
+    assert a.free_blocks == 59 and a.reserved == 0
