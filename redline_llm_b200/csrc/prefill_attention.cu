@@ -886,11 +886,16 @@ double SimulatedMakespan(const Chunk& chunk, int split_blocks, int sm_count, std
 }
 
 int ChooseSplitBlocks(const Chunk& chunk, int sm_count) {
+  // The last few choices: layers of one model may alternate between window and full attention, or between windows, and a
+  // replay takes as long as the kernel (2048 rows at 6144 both ways: 87 us a pair of calls if only the last was kept).
   struct Memo { Chunk chunk; int sms, choice; };
-  static Memo memo = {{-1, -1, -1, -1, -1}, -1, 0};
+  constexpr int kMemos = 8;
+  static Memo memos[kMemos] = {};   // (a chunk of no rows is never asked for)
+  static int oldest = 0;
   static std::mutex memo_mutex;
   std::lock_guard<std::mutex> lock(memo_mutex);
-  if (memo.chunk == chunk && memo.sms == sm_count) return memo.choice;
+  for (const Memo& memo : memos)
+    if (memo.chunk == chunk && memo.sms == sm_count) return memo.choice;
   const int n_tiles = chunk.Tiles(), heads = chunk.heads;
   int max_blocks = 1;
   for (int t = 0; t < n_tiles; ++t) max_blocks = std::max(max_blocks, chunk.Blocks(t));
@@ -912,7 +917,8 @@ int ChooseSplitBlocks(const Chunk& chunk, int sm_count) {
     for (int r : {2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32}) consider((max_blocks + r - 1) / r);   // equal cuts of the longest tile
     for (int run = max_blocks - 4; run > max_blocks / 2; run -= 4) consider(run);                   // cuts that only the longer tiles get
   }
-  memo = {chunk, sm_count, best};
+  memos[oldest] = {chunk, sm_count, best};
+  oldest = (oldest + 1) % kMemos;
   return best;
 }
 

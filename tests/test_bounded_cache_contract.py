@@ -1,6 +1,7 @@
 """The bounded-cache launchers' refusals and host arithmetic, through the C ABI without a device: every call here is
 answered before anything is launched."""
 import ctypes as C
+import time
 
 import pytest
 
@@ -192,3 +193,27 @@ def test_weights_must_cover_the_pool_and_tables_and_lengths_be_int32():
     K._rows_fit(wide[:, 4 * d:], rows, 16 * d, 12 * d)
     with pytest.raises(K.KernelError, match="out must hold"):
         K._rows_fit(wide[:, 5 * d:], rows, 16 * d, 12 * d)
+
+
+def test_prompt_launch_plans_are_remembered_for_layers_that_alternate():
+    """A launch plan is worked out by replaying the launch, which takes as long as the kernel it is for. Window and full
+    attention in turn, or several windows, each find theirs again."""
+    def full():
+        K.prefill_attention_run_length(6144, 2048, 12, 148)
+
+    def window(w):
+        K.window_prefill_workspace_bytes(6144, 2048, 12, w, 4)
+
+    def host_us(calls, n=40):
+        best = float("inf")
+        for _ in range(5):
+            t = time.perf_counter()
+            for _ in range(n):
+                for f in calls:
+                    f()
+            best = min(best, time.perf_counter() - t)
+        return best / (n * len(calls)) * 1e6
+
+    calls = [full, lambda: window(1024), lambda: window(512), lambda: window(4096)]
+    alone = max(host_us([f]) for f in calls)
+    assert host_us(calls) < 4 * alone + 4
