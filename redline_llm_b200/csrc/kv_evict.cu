@@ -56,6 +56,7 @@ constexpr int kMaxListed = 1024;   // candidates of a bin that are taken out of 
 constexpr int kRanked = 64;        // of those, as many as are simply ranked against one another
 constexpr int kLoadAhead = 8;      // quads of weights a thread has in flight
 constexpr int kMaxCachedKeys = 45 * 1024;   // 180 KB
+constexpr int kPairKeys = 22 * 1024;        // two CTAs' keys fit an SM beside 24 KB each of everything else
 
 // What the CTAs of a cluster tell one another.
 struct Shared {
@@ -87,11 +88,13 @@ __device__ __forceinline__ int2 LoadPeer2(const int* mine, int rank) {   // two 
 }
 
 // Grid: (sequences * cluster, KV heads). CTA `rank` of an item's cluster has every quad of tokens of its slice. 1024 threads
-// where a CTA has its SM to itself; 512, without clusters, where there are more items than SMs and CTAs share one.
+// where a CTA has its SM to itself; 512, without clusters, where there are more items than SMs and two CTAs share one.
 template <int kSelectThreads>
 __global__ void __launch_bounds__(kSelectThreads, 1024 / kSelectThreads) SelectKernel(const Params p, int cluster) {
   constexpr int kSelectWarps = kSelectThreads / 32, kListed = kSelectThreads, kPerThread = kBins / kSelectThreads;
   static_assert(kListed <= kMaxListed && kPerThread % 2 == 0, "a thread per listed key, pairs of bins");
+  static_assert(2 * (kPairKeys * 4 + sizeof(Shared) + (kListed + 4 + kBins + 4 * kSelectWarps + 8) * 4 + 1024) <= 228 * 1024 || kSelectThreads > 512,
+                "two CTAs share an SM");
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ __align__(16) Shared sh;
   __shared__ __align__(16) uint32_t crowd[kListed + 4];
@@ -574,9 +577,11 @@ extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int
   const int sm_count = CurrentDeviceFacts().sm_count;
   int cluster = 1;
   while (cluster < kMaxSelectCluster && 2 * cluster * items <= sm_count && tokens / (2 * cluster) >= 2048) cluster *= 2;
-  // More items than SMs: half the threads, so that several CTAs share an SM and wait for their loads side by side (57 x 8 items of
-  // 425-9779 tokens: 27.0 us with the move, with 1024 threads each 32.6).
-  const bool crowded = items > sm_count;
+  // More items than SMs: half the threads, so that two CTAs share an SM and wait for their loads side by side (57 x 8 items of
+  // 425-9779 tokens: 27.0 us with the move, with 1024 threads each 32.6) - as long as the table's width lets the keys of two
+  // into its shared memory. Wider ones have an SM each in either form, and then all threads help (20 x 8 items of 30000-32768:
+  // 47.7 us, with 512 threads 58.2; the 57 x 8 in a table of 32768: 32.8 and 34.0).
+  const bool crowded = items > sm_count && p.cached_keys <= kPairKeys;
   const size_t key_bytes = static_cast<size_t>(p.cached_keys) * 4;
   const dim3 select_grid(static_cast<unsigned>(num_seqs) * cluster, num_kv_heads);
   cudaError_t e = crowded ? LaunchDependent(SelectKernel<512>, select_grid, dim3(512), key_bytes, 1, s, p, 1)

@@ -563,6 +563,13 @@ def test_evict_more_tokens_than_shared_memory_holds():
     check_evict(c, 40000, 0, 0, some_weights(c, "ties"), True)
 
 
+@pytest.mark.parametrize("spare", [0, 1400, 1500, 2600])
+def test_evict_more_items_than_sms_in_tables_of_any_width(spare):
+    """160 items in tables whose width lets two selections share an SM or not, and behind what shared memory holds."""
+    c = Cache([40 + 13 * i for i in range(20)], 8, seed=spare, spare=spare)
+    check_evict(c, 150, 4, 30, some_weights(c, "spread"), True)
+
+
 @pytest.mark.parametrize("head_dim", [8, 64, 96, 256, 1024])
 def test_evict_row_widths(head_dim):
     c = Cache([90, 200], 3, seed=head_dim, extra_pages=40, head_dim=head_dim)
