@@ -344,7 +344,8 @@ int rl_decode_linear_set_max_splits(int max_splits);
  * `window` tokens up to and including p:  V(p) = { t <= p : t < sinks or t > p - window }  (window >= 1, sinks >= 0;
  * a window that covers the sequence is plain causal attention). Shared by the three attention launchers below:
  * head_dim 128, 1 to 8 KV heads with 1 to 8 query heads each, scale positive and finite, FP32 scores, statistics and
- * accumulation, masking by SELECT (what a slot that no row of the call sees holds - NaN included - reaches no result), one
+ * accumulation, probabilities rounded to FP16 for the product with V (as in the full kernels; one below 2^-14 of its
+ * row's largest is off by up to 2^-25 of that), masking by SELECT (what a slot that no row of the call sees holds - NaN included - reaches no result), one
  * FP16 rounding of the output; out overlaps neither q nor the pool. Pages that hold no visible token are not read, and
  * neither are their block-table entries: a caller may have given them to other sequences. None of the four has a counterpart in the reference (full causal attention over
  * a cache that only grows, src/kernels/kernels.cuh:125-187 there).

@@ -58,9 +58,17 @@ inline cudaError_t LaunchOverlapped(void (*kernel)(KArgs...), dim3 grid, dim3 bl
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// A dependent launch whatever the switch says, for kernels that touch nothing before griddepcontrol.wait and whose
-// every block executes it: the launch is set up under the tail of the stream's previous kernel, and no order that an
-// ordinary launch would keep is lost. cluster_x > 1: thread-block clusters of that many neighbours along x.
+// A dependent launch whatever the switch says: it is set up, and may start, under the tail of the stream's previous kernel.
+// Every block executes griddepcontrol.wait, so that no grid ends ahead of the one before it, and no order that an ordinary
+// launch would keep is lost as long as what a kernel touches before that wait is nothing that a kernel which may still be
+// running writes. Which kernels may is decided by where the PREVIOUS one releases its dependents:
+//  * prompt attention with a window, selection and move of an eviction, decode without the overlap option: nothing before it;
+//  * decode under the overlap option (run_ahead): lengths, tables and all but the newest pages. The option's rules keep other
+//    kernels in flight from writing those; the eviction's move, which does write them, releases its dependents last;
+//  * adding up the weights: lengths, tables and old weights. The decode kernel ahead of it writes none of them and releases
+//    it only behind its own wait, when whatever came before is done.
+// A new kernel that writes any of these and releases its dependents early would break the ones that read them.
+// cluster_x > 1: thread-block clusters of that many neighbours along x.
 template <typename... KArgs, typename... Args>
 inline cudaError_t LaunchDependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster_x,
                                    cudaStream_t stream, Args&&... args) {

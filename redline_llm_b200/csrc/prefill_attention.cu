@@ -48,7 +48,8 @@
 //  * With a sliding window and sinks (rl_launch_paged_window_prefill_attention) the same kernel, instantiated over a tile's
 //    LIST of visible pages (SpanOfTile below) instead of all pages up to the diagonal: rows mask by position in the blocks
 //    that hold an edge of the window, V rows that no row of the tile sees are cleared, everything else is as above. 2048 rows
-//    at context 8192 with a window of 1024: 35 us; 8192 rows with a window of 4096: 178 us, 880 TFLOP/s of visible pairs.
+//    at context 8192 with a window of 1024: 35 us; 8192 rows with a window of 4096: 178 us, 880 TFLOP/s of visible pairs, replayed
+//    from a graph over three inputs, and 195-199 us, 790-805 TFLOP/s, as separate calls one after the other (power cap).
 //    Short windows are bound by a CTA's fixed 8 us and by 192 items on 148 SMs (ten blocks each), long ones by a block's softmax.
 // Every mbarrier wait is bounded and reports through rl_prefill_attention_health.
 #include <cuda.h>

@@ -13,8 +13,9 @@
 //    64 sequences with a window of 4096 and 16 sinks: 45.4 us, 5.7 TB/s. What is left around the stream is a chain of
 //    ~6 us - lengths, table, first pages; fold, record, ticket, merge - which is all there is to a small call (300 tokens: 6.3 us).
 //  * S^T = K.Q^T and O^T = V^T.P^T on mma.sync m16n8k16: 16 tokens of a page fill M, the group's queries fill N = 8.
-//    The online softmax keeps FP32 maxima and sums; probabilities go to FP16 for P.V (relative 2^-12 on average, the
-//    size of the output's own rounding), their sum is taken before that rounding.
+//    The online softmax keeps FP32 maxima and sums; probabilities go to FP16 for P.V (off by half a step, at most 2^-11
+//    relative like the output's own rounding, and by up to 2^-25 of a row's largest where that falls below FP16's normal range);
+//    their sum is taken before that rounding. Against 64 bits the outputs are off by 2.6e-4 of their size, 2.1e-4 with P in 32 bits.
 //  * An item cut by a share boundary leaves (o, m, l) records in the workspace; whoever of its contributors arrives last
 //    folds them in CTA order, so the result does not depend on who that is. A contributor that finds all others already
 //    there - usual at the end of a share, whose neighbour met the item first thing - reads them straight away.
@@ -51,7 +52,7 @@ constexpr int kMergeBatch = 16;      // longer ones: records in flight per threa
 constexpr int kMinPagesPerCta = kWarps;
 constexpr int kMinChunk = 2 * kWarps;      // an item is not cut finer than this ...
 constexpr int kWholeItem = 3 * kWarps;     // ... and not at all up to this: a ring holds three pages per warp, and handing over
-                                           // costs 1 us (300 tokens: 6.65 us whole, 7.73 in two; 8000 tokens: 11.5 us in
+                                           // costs 1 us (300 tokens take 1.1 us longer in two; 8000 tokens: 11.5 us in
                                            // chunks of 16 pages, 14.8 in chunks of 8, 11.6 in chunks of 32)
 constexpr int kTeamPages = 32;            // pages of an item that one warp of a team may take: their tile indices sit one per lane
 constexpr int kSegmentPages = 12;    // what a second item costs a CTA (fold and hand-over, 2-3 us), in pages
