@@ -604,7 +604,8 @@ extern "C" int rl_launch_kv_evict(void* kv_pool_layer, float* weights, const int
   // 256 rows in the registers of each CTA, so up to 2048 a round; where the items fill the machine several times over, small CTAs, four
   // to an SM, whose rounds overlap (one sequence of 32768 tokens to 8192: 36.0 us wide, 46.9 small; 5 x 4 items of 16000-32768 to 4099,
   // clusters of four: 42.3 against 50.0; 64 sequences to 2048 stay small: 52.6). And no more CTAs than one round of the longest
-  // item fills (57 x 8 items to 12 tokens: 26.4 us, in clusters of eight 39.4).
+  // item fills (57 x 8 items to 12 tokens: 26.4 us, in clusters of eight 39.4). (Both sides from when the move released its
+  // dependents at its start; the forms chosen now take 36.4, 42.8, 54.6 and 27.1 us, one launch behind the other.)
   int cluster_size = kCluster;
   while (cluster_size > 4 && items * cluster_size > sms) cluster_size /= 2;
   const bool wide = in_place && items * cluster_size <= sms;
