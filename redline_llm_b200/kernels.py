@@ -263,13 +263,15 @@ def _holds(name: str, t, dtype: str, at_least: int) -> None:
 def _rows_fit(t, rows: int, stride: int, width: int) -> None:
     """The output rows of a bounded-cache attention launcher: 16-bit elements, the last row inside the tensor's memory."""
     need = (rows - 1) * stride + width
-    if t.element_size() != 2 or (rows > 0 and t.numel() < need
+    if t.element_size() != 2 or (rows > 0 and (t.numel() < need or not t.is_contiguous())   # a view: what is behind it counts
                                  and t.untyped_storage().nbytes() // 2 - t.storage_offset() < need):
         raise KernelError(f"out must hold {rows} rows of {width} 16-bit elements at a stride of {stride}")
 
 
 def _weights_fit(weights, kv_pool_layer, head_dim: int) -> None:
     """One weight per K row of the pool: the kernels find both by the same page numbers."""
+    if not kv_pool_layer.is_contiguous():
+        raise KernelError("kv_pool_layer must be contiguous: pages are found by their number")
     _holds("weights", weights, "float32", kv_pool_layer.nbytes // (4 * head_dim) if head_dim > 0 else 1)
 
 
