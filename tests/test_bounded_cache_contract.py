@@ -191,7 +191,7 @@ def test_weights_must_cover_the_pool_and_tables_and_lengths_be_int32():
     wide = torch.zeros(rows, 16 * d, dtype=torch.float16)
     K._rows_fit(wide[:, :12 * d], rows, 16 * d, 12 * d)
     K._rows_fit(wide[:, 4 * d:], rows, 16 * d, 12 * d)
-    for short in (wide[:, 5 * d:], wide[:1].expand(rows, 16 * d)):
+    for short in (wide[:, 5 * d:], wide[:1].clone().expand(rows, 16 * d)):
         with pytest.raises(K.KernelError, match="out must hold"):
             K._rows_fit(short, rows, 16 * d, 12 * d)
     for call in (evict, weights):
